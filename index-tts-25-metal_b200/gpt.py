@@ -113,6 +113,12 @@ SIGNATURES = {
     "itts_qwen_last_timing": (C.c_int, [_P, _P]),
     "itts_codec_last_timing": (C.c_int, [_P, _P]),
     "itts_codec_set_gemm_mode": (C.c_int, [_P, C.c_int]),
+    # include/itts_paged.h (argument structs in paged.py)
+    "itts_paged_last_error": (C.c_char_p, []),
+    "itts_paged_tables": (C.c_int, [C.c_int, _P, _P]),
+    "itts_paged_append": (C.c_int, [C.c_int, _P, _P]),
+    "itts_paged_attention": (C.c_int, [C.c_int, _P, _P]),
+    "itts_paged_attention_workspace": (C.c_size_t, [C.c_int32]),
 }
 
 _lib = None
