@@ -1,0 +1,297 @@
+// What the paged attention kernels share: the geometry of a request, the
+// sharing-out of the work among CTAs, and the partial results of items that
+// several CTAs work on.
+//
+// An item is (request, row tile, key / value head): the rows of a request that
+// read one key / value head, G = q_heads / heads of them per token, are
+// numbered token-major (row r = token r / G, query head h * G + r % G) and cut
+// into tiles of RT rows, so that the query heads of a group share the keys they
+// load.  An item's keys (those that its last row sees) are cut into units of KU
+// keys; an item without keys has one unit, which writes its zeros.  The lengths
+// are on the device, so the sharing-out is too: every CTA adds up the units of
+// all requests and takes an equal share [i U / n, (i + 1) U / n) of them, which
+// keeps all SMs busy whether there are many short requests or one long one.
+// An item that ends up with several CTAs leaves partial sums in the workspace,
+// two slots a CTA (slot 0: the item its share begins inside of; slot 1: the
+// item that begins in it and goes on in the next); k_join adds them up in CTA
+// order, so results do not depend on timing.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "paged.hpp"
+
+namespace itts {
+namespace paged {
+
+constexpr int kMaxCtas = 592;  // of one attention launch: 148 SMs, up to four CTAs each
+constexpr float kLog2e = 1.4426950408889634f;
+
+// The part of the arguments that the kernels read.
+struct Attn {
+    itts_paged_cache c;
+    const void* q;
+    void* out;
+    long long q_row, q_head, o_row, o_head;
+    const int *q_start, *lens, *table;
+    long long table_stride;
+    int rows, requests, group, shift;  // group = q_heads / heads, shift = log2(block_size)
+    int cap;                           // keys that the table's columns can name
+    int above;                         // requests of more than this many rows (per kv head) ...
+    int below;                         // ... and up to this many are this kernel's
+    float scale2;                      // |scale| log2(e), at least 1e-30: a masked -inf stays -inf
+    float sign;                        // of the scale, taken into q
+    float* part;                       // partial sums
+    int4* rec;                         // per CTA: {CTAs of the item that begins here, first row, kv head, rows}
+};
+
+// A request's rows and keys.
+struct Request {
+    int start, tokens, rows, len;
+    __device__ __forceinline__ void load(const Attn& a, int b) {
+        const int s = __ldcg(a.q_start + b), e = __ldcg(a.q_start + b + 1);
+        len = max(__ldcg(a.lens + b), 0);
+        start = min(max(s, 0), a.rows);
+        tokens = max(min(max(e, 0), a.rows) - start, 0);
+        const long long r = (long long)tokens * a.group;
+        rows = r > a.above && r <= a.below ? int(r) : 0;
+    }
+    // Position of the token of row r.
+    __device__ __forceinline__ int pos(const Attn& a, int r) const { return len - tokens + r / a.group; }
+    // Keys that some row of tile t sees.
+    template <int RT>
+    __device__ __forceinline__ int keys(const Attn& a, int t) const {
+        const int last = pos(a, min((t + 1) * RT, rows) - 1);
+        return min(max(last + 1, 0), a.cap);
+    }
+    template <int RT, int KU>
+    __device__ __forceinline__ int units(const Attn& a, int t) const {
+        return max(1, (keys<RT>(a, t) + KU - 1) / KU);
+    }
+    // Units of one key / value head over all tiles.
+    template <int RT, int KU>
+    __device__ __forceinline__ long long total(const Attn& a) const {
+        long long n = 0;
+        for (int t = 0; t * RT < rows; ++t) n += units<RT, KU>(a, t);
+        return n;
+    }
+};
+
+// The units of a launch and where this CTA's share begins.
+struct Share {
+    long long units, u0, u1;  // of all items; this CTA's
+    int ctas;                 // that have a share: every one of them at least one unit
+    int b;                    // request of u0
+    long long base;           // units before that request
+};
+
+template <int kThreadsT>
+struct PlanSmem {
+    long long sum[kThreadsT];
+    long long warp_sum[kThreadsT / 32 + 1];
+    Share share;
+};
+
+// Called by all threads of the CTA.  `ctas` is what the launch may use; with
+// few units the last CTAs get none.
+template <int RT, int KU, int kThreadsT>
+__device__ Share plan(const Attn& a, int cta, int ctas, PlanSmem<kThreadsT>& sm) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int per = (a.requests + kThreadsT - 1) / kThreadsT, b0 = tid * per;
+    long long mine = 0;
+    for (int b = b0; b < min(a.requests, b0 + per); ++b) {
+        Request r;
+        r.load(a, b);
+        mine += r.total<RT, KU>(a);
+    }
+    mine *= a.c.heads;
+    long long inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+    }
+    if (lane == 31) sm.warp_sum[warp] = inc;
+    __syncthreads();
+    long long before = inc - mine, all = 0;
+#pragma unroll
+    for (int w = 0; w < kThreadsT / 32; ++w) {
+        if (w < warp) before += sm.warp_sum[w];
+        all += sm.warp_sum[w];
+    }
+    Share s;
+    s.units = all;
+    s.ctas = int(min((long long)ctas, all));
+    s.u0 = cta < s.ctas ? all * cta / s.ctas : all;
+    s.u1 = cta < s.ctas ? all * (cta + 1) / s.ctas : all;
+    s.b = 0;
+    s.base = 0;
+    if (tid == 0) sm.share = s;
+    __syncthreads();
+    if (mine > 0 && before <= s.u0 && s.u0 < before + mine) {  // one thread holds the request of u0
+        s.base = before;
+        for (s.b = b0;; ++s.b) {
+            Request r;
+            r.load(a, s.b);
+            const long long n = r.total<RT, KU>(a) * a.c.heads;
+            if (s.u0 < s.base + n) break;
+            s.base += n;
+        }
+        sm.share = s;
+    }
+    __syncthreads();
+    return sm.share;
+}
+
+// Walks the items of a share, unit by unit.
+template <int RT, int KU>
+struct Walk {
+    Request r;
+    int b, t, h;      // item: request, tile, kv head
+    int k, nk;        // unit of the item, units of the item
+    __device__ __forceinline__ void start(const Attn& a, const Share& s) {
+        b = s.b;
+        r.load(a, b);
+        t = 0;
+        long long left = s.u0 - s.base;
+        for (;; ++t) {
+            nk = r.units<RT, KU>(a, t);
+            if (left < (long long)nk * a.c.heads) break;
+            left -= (long long)nk * a.c.heads;
+        }
+        h = int(left / nk);
+        k = int(left - (long long)h * nk);
+    }
+    // To the first unit of the next item (there is one).
+    __device__ __forceinline__ void next(const Attn& a) {
+        k = 0;
+        if (++h < a.c.heads) return;
+        h = 0;
+        ++t;
+        if (t * RT >= r.rows) {
+            t = 0;
+            do r.load(a, ++b);
+            while (r.rows == 0);
+        }
+        nk = r.units<RT, KU>(a, t);
+    }
+};
+
+// The CTA whose share holds unit u.
+__device__ __forceinline__ int cta_of(const Share& s, long long u) {
+    int i = int(u * s.ctas / s.units);
+    while (i > 0 && s.units * i / s.ctas > u) --i;
+    while (i + 1 < s.ctas && s.units * (i + 1) / s.ctas <= u) ++i;
+    return i;
+}
+
+// Partial sums of an item: RT rows of D unnormalised outputs, then RT pairs
+// (maximum in units of log2, sum).
+template <int RT, int D>
+__host__ __device__ constexpr size_t part_floats() {
+    return size_t(RT) * (D + 2);
+}
+template <int RT, int D>
+__device__ __forceinline__ float* part_slot(const Attn& a, int cta, int which) {
+    return a.part + (size_t)(2 * cta + which) * part_floats<RT, D>();
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <class T>
+__device__ __forceinline__ void store4(T* p, float4 v);
+template <>
+__device__ __forceinline__ void store4<float>(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
+template <>
+__device__ __forceinline__ void store4<__half>(__half* p, float4 v) {
+    const __half2 x = __floats2half2_rn(v.x, v.y), y = __floats2half2_rn(v.z, v.w);
+    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+}
+template <>
+__device__ __forceinline__ void store4<__nv_bfloat16>(__nv_bfloat16* p, float4 v) {
+    const __nv_bfloat162 x = __floats2bfloat162_rn(v.x, v.y), y = __floats2bfloat162_rn(v.z, v.w);
+    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+}
+
+// Where row `row` of the item whose first row is `first` (counted over a
+// request that starts at `start`) goes.
+template <class T>
+__device__ __forceinline__ T* out_row(const Attn& a, int start, int first, int row, int kvh) {
+    const int r = first + row, tok = r / a.group, g = r - tok * a.group;
+    return static_cast<T*>(a.out) + (long long)(start + tok) * a.o_row + (long long)(kvh * a.group + g) * a.o_head;
+}
+
+__device__ __forceinline__ float4 normalised(float4 o, float l) {
+    if (l == 0.f) return make_float4(0.f, 0.f, 0.f, 0.f);  // no key: a NaN sum is not 0
+    const float i = 1.0f / l;
+    return make_float4(o.x * i, o.y * i, o.z * i, o.w * i);
+}
+
+// Adds up the partial sums of the items that several CTAs worked on: CTA i
+// takes the item that begins in share i, if it goes on in other shares.
+constexpr int kJoinThreads = 256;
+template <class T, int RT, int D>
+__global__ void __launch_bounds__(kJoinThreads) k_join(Attn a) {
+    pdl_wait();
+    pdl_trigger();
+    const int cta = blockIdx.x;
+    const int4 rec = __ldcg(a.rec + 2 * cta);
+    if (rec.x < 2) return;
+    const int4 where = __ldcg(a.rec + 2 * cta + 1);
+    const int parts = rec.x, rows = rec.w, kvh = rec.z, start = where.x, first = where.y;
+    extern __shared__ float4 joined[];
+    // groups of D / 4 threads: each takes every gth part of a row
+    constexpr int kCols = D / 4, kGroups = kJoinThreads / kCols;
+    const int col = threadIdx.x % kCols, grp = threadIdx.x / kCols;
+    __shared__ float wl[kGroups][2];
+    const auto slot = [&](int i) { return part_slot<RT, D>(a, cta + i, i == 0 ? 1 : 0); };
+    for (int row = 0; row < rows; ++row) {
+        float m = -INFINITY, l = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = grp; i < parts; i += kGroups) {
+            const float* p = slot(i);
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p + RT * D) + row);
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(p + row * D) + col);
+            const float mn = fmaxf(m, ml.x), ref = mn == -INFINITY ? 0.f : mn;
+            const float f = ex2(m - ref), g = ex2(ml.x - ref);
+            l = l * f + ml.y * g;
+            o = make_float4(o.x * f + v.x * g, o.y * f + v.y * g, o.z * f + v.z * g, o.w * f + v.w * g);
+            m = mn;
+        }
+        joined[threadIdx.x] = o;
+        if (col == 0) {
+            wl[grp][0] = m;
+            wl[grp][1] = l;
+        }
+        __syncthreads();
+        if (grp == 0) {
+            float M = -INFINITY, L = 0.f;
+            for (int i = 0; i < kGroups; ++i) M = fmaxf(M, wl[i][0]);
+            const float ref = M == -INFINITY ? 0.f : M;
+            o = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int i = 0; i < kGroups; ++i) {
+                const float g = ex2(wl[i][0] - ref);
+                const float4 v = joined[i * kCols + col];
+                L += wl[i][1] * g;
+                o = make_float4(o.x + v.x * g, o.y + v.y * g, o.z + v.z * g, o.w + v.w * g);
+            }
+            store4<T>(out_row<T>(a, start, first, row, kvh) + 4 * col, normalised(o, L));
+        }
+        __syncthreads();
+    }
+}
+
+// Records the item that begins in this share and goes on (or none), for k_join.
+__device__ __forceinline__ void put_record(const Attn& a, int cta, int parts, int kvh, int rows, int start, int first) {
+    a.rec[2 * cta] = make_int4(parts, 0, kvh, rows);
+    a.rec[2 * cta + 1] = make_int4(start, first, 0, 0);
+}
+
+}  // namespace paged
+}  // namespace itts
