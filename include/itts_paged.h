@@ -145,7 +145,7 @@ typedef struct itts_paged_attention_args {
     const void* q;   /* [rows][q_heads][head_dim] of the cache's type, head_dim contiguous */
     void* out;       /* as q; must not overlap it unless it is q with the same strides */
     int32_t q_heads; /* a multiple of cache.heads, at most 128 times it */
-    int32_t rows;    /* 0 .. 2^30 */
+    int32_t rows;    /* 0 .. 2^30, and so is rows * q_heads / heads */
     int64_t q_row_stride, q_head_stride; /* elements */
     int64_t out_row_stride, out_head_stride;
     const int32_t* q_start; /* [requests + 1] */

@@ -151,6 +151,7 @@ int itts_paged_attention(int device, const itts_paged_attention_args* a, void* s
         check(a->rows >= 0 && a->rows <= kMaxRows, "rows out of range");
         check(a->q_heads >= 1 && a->q_heads % a->cache.heads == 0 && a->q_heads / a->cache.heads <= 128,
               "q_heads must be a multiple (at most 128 times) of the cache's heads");
+        check(int64_t(a->rows) * (a->q_heads / a->cache.heads) <= kMaxRows, "rows out of range");
         check(a->max_fresh >= 1, "max_fresh must be positive");
         check(std::isfinite(a->scale), "scale must be finite");
         check(a->workspace && aligned(a->workspace, 256) &&

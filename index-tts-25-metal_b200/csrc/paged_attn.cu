@@ -1,6 +1,6 @@
 // Causal attention of a step's fresh rows over a paged K/V cache
 // (itts_paged_attention): the choice of kernel and the workspace.
-#include <climits>
+#include <algorithm>
 #include <cmath>
 
 #include "paged_attn.cuh"
@@ -10,12 +10,18 @@ namespace paged {
 
 size_t few_workspace_floats(int head_dim);
 cudaError_t launch_few(const Attn& a, cudaStream_t s);
+size_t tile_workspace_floats(int head_dim);
+cudaError_t launch_tile(const Attn& a, cudaStream_t s);
 
 namespace {
+// Rows of a request and kv head up to which the streaming kernel is used.
+constexpr int kFewMost = 16;
 constexpr size_t kRecords = size_t(2) * kMaxCtas * sizeof(int4);
 }
 
-size_t attention_workspace(int head_dim) { return kRecords + few_workspace_floats(head_dim) * sizeof(float); }
+size_t attention_workspace(int head_dim) {
+    return kRecords + std::max(few_workspace_floats(head_dim), tile_workspace_floats(head_dim)) * sizeof(float);
+}
 
 cudaError_t launch_attention(const itts_paged_attention_args& p, cudaStream_t s) {
     Attn a{};
@@ -39,8 +45,10 @@ cudaError_t launch_attention(const itts_paged_attention_args& p, cudaStream_t s)
     a.sign = p.scale < 0.f ? -1.f : 1.f;
     a.rec = static_cast<int4*>(p.workspace);
     a.part = reinterpret_cast<float*>(static_cast<char*>(p.workspace) + kRecords);
-    a.above = 0;
-    a.below = INT_MAX;
+    if (p.cache.type != ITTS_PAGED_F32 && (long long)p.max_fresh * a.group > kFewMost) {
+        const cudaError_t e = launch_tile(a, s);
+        if (e != cudaErrorNotSupported) return e;
+    }
     return launch_few(a, s);
 }
 

@@ -39,8 +39,6 @@ struct Attn {
     long long table_stride;
     int rows, requests, group, shift;  // group = q_heads / heads, shift = log2(block_size)
     int cap;                           // keys that the table's columns can name
-    int above;                         // requests of more than this many rows (per kv head) ...
-    int below;                         // ... and up to this many are this kernel's
     float scale2;                      // |scale| log2(e), at least 1e-30: a masked -inf stays -inf
     float sign;                        // of the scale, taken into q
     float* part;                       // partial sums
@@ -55,8 +53,7 @@ struct Request {
         len = max(__ldcg(a.lens + b), 0);
         start = min(max(s, 0), a.rows);
         tokens = max(min(max(e, 0), a.rows) - start, 0);
-        const long long r = (long long)tokens * a.group;
-        rows = r > a.above && r <= a.below ? int(r) : 0;
+        rows = tokens * a.group;  // the host has checked that a.rows * group <= 2^30
     }
     // Position of the token of row r.
     __device__ __forceinline__ int pos(const Attn& a, int r) const { return len - tokens + r / a.group; }
@@ -89,7 +86,6 @@ struct Share {
 
 template <int kThreadsT>
 struct PlanSmem {
-    long long sum[kThreadsT];
     long long warp_sum[kThreadsT / 32 + 1];
     Share share;
 };
@@ -285,6 +281,34 @@ __global__ void __launch_bounds__(kJoinThreads) k_join(Attn a) {
         }
         __syncthreads();
     }
+}
+
+// The same for items of many rows, which few CTAs share: a thread per four
+// columns of a row, blockIdx.y over the rows.
+__host__ __device__ constexpr int join_rows(int D) { return kJoinThreads * 4 / D; }
+template <class T, int RT, int D>
+__global__ void __launch_bounds__(kJoinThreads) k_join_rows(Attn a) {
+    pdl_wait();
+    pdl_trigger();
+    const int cta = blockIdx.x;
+    const int4 rec = __ldcg(a.rec + 2 * cta);
+    const int col = threadIdx.x % (D / 4), row = blockIdx.y * join_rows(D) + threadIdx.x / (D / 4);
+    if (rec.x < 2 || row >= rec.w) return;
+    const int4 where = __ldcg(a.rec + 2 * cta + 1);
+    float m = -INFINITY, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int i = 0; i < rec.x; ++i) {
+        const float* p = part_slot<RT, D>(a, cta + i, i == 0 ? 1 : 0);
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(p + RT * D) + row);
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(p + row * D) + col);
+        const float mn = fmaxf(m, ml.x), ref = mn == -INFINITY ? 0.f : mn;
+        const float f = ex2(m - ref), g = ex2(ml.x - ref);
+        l = l * f + ml.y * g;
+        o = make_float4(o.x * f + v.x * g, o.y * f + v.y * g, o.z * f + v.z * g, o.w * f + v.w * g);
+        m = mn;
+    }
+    store4<T>(out_row<T>(a, where.x, where.y, row, rec.z) + 4 * col, normalised(o, l));
 }
 
 // Records the item that begins in this share and goes on (or none), for k_join.

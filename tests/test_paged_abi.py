@@ -124,6 +124,7 @@ def test_append_refusals(lib, gpt_mod, paged, field, value, text):
     ("q_heads", 0, "q_heads"),
     ("q_heads", 258, "q_heads"),
     ("rows", -1, "rows out of range"),
+    ("rows", (1 << 29) + 1, "rows out of range"),
     ("q_start", None, "null argument"),
     ("lens", None, "null argument"),
     ("table", None, "block table is null"),
