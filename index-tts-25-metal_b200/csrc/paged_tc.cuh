@@ -47,6 +47,15 @@ __device__ __forceinline__ bool mbar_wait(unsigned long long* bar, uint32_t pari
     }
 }
 
+// The same value in every lane, and known to be: the products' operands then
+// stay in uniform registers.
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+__device__ __forceinline__ bool elect() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
 // One block's rows of one head, 128 bytes of each (x: first element).
 __device__ __forceinline__ void tma_block(uint32_t dst, const CUtensorMap* map, int x, int head, int block,
                                           unsigned long long* bar) {
@@ -57,6 +66,16 @@ __device__ __forceinline__ void tma_block(uint32_t dst, const CUtensorMap* map, 
         : "memory");
 }
 
+// A box of query rows (tokens x heads), 128 bytes of each.
+__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, int x, int head, int token,
+                                         unsigned long long* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+        "[%5];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(token), "r"(smem_u32(bar))
+        : "memory");
+}
+
 __device__ __forceinline__ void tc_commit(unsigned long long* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                  : "memory");
@@ -64,15 +83,24 @@ __device__ __forceinline__ void tc_commit(unsigned long long* bar) {
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// ... that also ties the registers that the loads fill to the wait: no use of them moves above it.
+template <int N>
+__device__ __forceinline__ void tc_wait_ld(uint32_t (&v)[N]) {
+    tc_wait_ld();
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+r"(v[i]));
+}
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Shared-memory descriptors, 128-byte swizzle (rows of 128 bytes, groups of
 // eight rows 1024 bytes apart), descriptor version 1.  K-major operand: rows
 // are the M or N index.  MN-major: rows are the K index, `lead` bytes between
-// the blocks of 64 M or N elements.
-__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr, uint32_t lead) {
-    return uint64_t((addr >> 4) & 0x3FFFu) | (uint64_t(lead >> 4) << 16) | (uint64_t(1024 >> 4) << 32) |
-           (uint64_t(1) << 46) | (uint64_t(2) << 61);
+// the blocks of 64 M or N elements.  The high word is the same for all; the low
+// word holds address / 16 and lead / 16, so stepping through an operand adds
+// to it.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_low(uint32_t addr, uint32_t lead) {
+    return ((addr >> 4) & 0x3FFFu) | ((lead >> 4) << 16);
 }
 
 #define ITTS_R32(v, o)                                                                                             \
@@ -105,6 +133,24 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&v)[N],
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
         "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::ITTS_S32(v, o),
         "r"(addr)
+        : "memory");
+}
+template <int N>
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&v)[N]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(addr));
+}
+template <int N>
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[N]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+        "%14, %15};" ::"r"(v[0]),
+        "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+        "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(addr)
         : "memory");
 }
 #undef ITTS_R32
