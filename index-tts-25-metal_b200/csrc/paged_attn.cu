@@ -12,6 +12,8 @@ size_t few_workspace_floats(int head_dim);
 cudaError_t launch_few(const Attn& a, cudaStream_t s);
 size_t tile_workspace_floats(int head_dim);
 cudaError_t launch_tile(const Attn& a, cudaStream_t s);
+size_t tile32_workspace_floats(int head_dim);
+cudaError_t launch_tile32(const Attn& a, cudaStream_t s);
 
 namespace {
 // Rows of a request and kv head up to which the streaming kernel is used.
@@ -20,7 +22,8 @@ constexpr size_t kRecords = size_t(2) * kMaxCtas * sizeof(int4);
 }
 
 size_t attention_workspace(int head_dim) {
-    return kRecords + std::max(few_workspace_floats(head_dim), tile_workspace_floats(head_dim)) * sizeof(float);
+    return kRecords + std::max({few_workspace_floats(head_dim), tile_workspace_floats(head_dim),
+                                tile32_workspace_floats(head_dim)}) * sizeof(float);
 }
 
 cudaError_t launch_attention(const itts_paged_attention_args& p, cudaStream_t s) {
@@ -45,7 +48,8 @@ cudaError_t launch_attention(const itts_paged_attention_args& p, cudaStream_t s)
     a.sign = p.scale < 0.f ? -1.f : 1.f;
     a.rec = static_cast<int4*>(p.workspace);
     a.part = reinterpret_cast<float*>(static_cast<char*>(p.workspace) + kRecords);
-    if (p.cache.type != ITTS_PAGED_F32 && (long long)p.max_fresh * a.group > kFewMost) {
+    if ((long long)p.max_fresh * a.group > kFewMost) {
+        if (p.cache.type == ITTS_PAGED_F32) return launch_tile32(a, s);
         const cudaError_t e = launch_tile(a, s);
         if (e != cudaErrorNotSupported) return e;
     }
