@@ -27,8 +27,8 @@ namespace {
 
 constexpr int kTabThreads = 512;
 constexpr int kTabWarps = kTabThreads / 32;
-constexpr int kFusedRows = 4096;  // rows that one launch maps
-constexpr int kSmallWork = 4096;  // requests + fused rows that one CTA handles
+constexpr int kFusedRows = 8192;  // rows that one launch maps
+constexpr int kSmallWork = 1024;  // requests, mapped rows and new blocks that one CTA handles
 constexpr int kClusterCtas = 8;
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -206,25 +206,50 @@ __global__ void __launch_bounds__(kTabThreads) k_tables(itts_paged_tables_args a
     if (ctas > 1) cluster_wait();
 }
 
-// Row maps from the finished tables: four rows per thread.
-__global__ void __launch_bounds__(256) k_slots(itts_paged_tables_args a) {
+// Row maps from the finished tables: four rows per thread, 1024 per block.  The
+// block finds its first row's request in two loads (256 samples of q_start, then
+// a window from the sampled request on), and its threads bisect the window in
+// shared memory.
+constexpr int kSlotThreads = 256, kWindow = 5 * kSlotThreads;
+__global__ void __launch_bounds__(kSlotThreads) k_slots(itts_paged_tables_args a) {
+    __shared__ int first[kWindow + 1], len[kWindow];
     pdl_wait();
-    const int t0 = (blockIdx.x * 256 + threadIdx.x) * 4;
+    const int B = a.requests, shift = 31 - __clz(a.block_size), tid = threadIdx.x;
+    const int block0 = blockIdx.x * kSlotThreads * 4, t0 = block0 + tid * 4;
+    const int total = __ldcg(a.q_start + B);
+    const int sample = int((long long)tid * B / kSlotThreads);
+    const int low = __syncthreads_count(__ldcg(a.q_start + sample) <= block0) - 1;
+    const int base = int((long long)low * B / kSlotThreads);  // its q_start is at or before the block
+#pragma unroll
+    for (int i = 0; i < kWindow; i += kSlotThreads) {
+        const int b = base + i + tid;
+        first[i + tid] = b < B ? __ldcg(a.q_start + b) : total;
+        len[i + tid] = b < B ? __ldcg(a.lens + b) : 0;
+    }
+    if (tid == 0) first[kWindow] = base + kWindow < B ? __ldcg(a.q_start + base + kWindow) : total;
+    __syncthreads();
     if (t0 >= a.rows) return;
-    const int B = a.requests, shift = 31 - __clz(a.block_size), total = __ldcg(a.q_start + B);
     int pos[4] = {0, 0, 0, 0}, slot[4] = {-1, -1, -1, -1};
     if (t0 < total) {
-        int b = owner([&](int r) { return __ldcg(a.q_start + r); }, B, t0), end = __ldcg(a.q_start + b + 1), len = __ldcg(a.lens + b);
+        // requests without rows may push the row's request out of the window
+        const bool near = t0 < first[kWindow];
+        int b = near ? base + owner([&](int r) { return first[r]; }, kWindow, t0)
+                     : owner([&](int r) { return __ldcg(a.q_start + r); }, B, t0);
+        const auto end_of = [&](int r) {
+            return r - base < kWindow ? first[r - base + 1] : __ldcg(a.q_start + r + 1);
+        };
+        const auto len_of = [&](int r) { return r - base < kWindow ? len[r - base] : __ldcg(a.lens + r); };
+        int end = end_of(b), n = len_of(b);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int t = t0 + k;
             if (t >= total) break;
             while (t >= end) {
                 ++b;
-                end = __ldcg(a.q_start + b + 1);
-                len = __ldcg(a.lens + b);
+                end = end_of(b);
+                n = len_of(b);
             }
-            pos[k] = len - (end - t);
+            pos[k] = n - (end - t);
             const int id = __ldcg(a.table + (long long)b * a.table_stride + (pos[k] >> shift));
             if ((unsigned)id < (unsigned)a.blocks) slot[k] = (id << shift) + (pos[k] & (a.block_size - 1));
         }
@@ -248,7 +273,7 @@ __global__ void __launch_bounds__(256) k_slots(itts_paged_tables_args a) {
 cudaError_t launch_tables(const itts_paged_tables_args& a, cudaStream_t s) {
     const bool fused = a.rows <= kFusedRows;
     const int map_rows = fused ? a.rows : 0;
-    const int ctas = a.requests + map_rows <= kSmallWork ? 1 : kClusterCtas;
+    const int ctas = a.requests + map_rows + a.rows / a.block_size <= kSmallWork ? 1 : kClusterCtas;
     const size_t smem = (size_t(a.requests) * 4 + 3) * sizeof(int);
     cudaError_t e = cudaSuccess;
     if (smem > 48 * 1024 &&
@@ -267,7 +292,7 @@ cudaError_t launch_tables(const itts_paged_tables_args& a, cudaStream_t s) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     if ((e = cudaLaunchKernelEx(&cfg, k_tables, a, ctas, map_rows)) != cudaSuccess || fused) return e;
-    return launch_pdl(k_slots, (a.rows + 1023) / 1024, 256, 0, s, a);
+    return launch_pdl(k_slots, (a.rows + 4 * kSlotThreads - 1) / (4 * kSlotThreads), kSlotThreads, 0, s, a);
 }
 
 }  // namespace paged
