@@ -20,11 +20,27 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "common.cuh"
 #include "paged.hpp"
 
 namespace itts {
 namespace paged {
+
+// Allows a kernel `bytes` of dynamic shared memory, once per device.
+template <auto kKernel>
+cudaError_t allow_smem(size_t bytes) {
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
 
 constexpr int kMaxCtas = 592;  // of one attention launch: 148 SMs, up to four CTAs each
 constexpr float kLog2e = 1.4426950408889634f;

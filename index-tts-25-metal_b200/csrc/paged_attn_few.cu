@@ -460,7 +460,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_attn_few(const __grid_consta
 
 template <class T, int D>
 cudaError_t launch(const Attn& a, cudaStream_t s) {
-    cudaError_t e = cudaFuncSetAttribute(k_attn_few<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kFewSmem));
+    cudaError_t e = allow_smem<k_attn_few<T, D>>(kFewSmem);
     if (e != cudaSuccess) return e;
     const int ctas = 2 * 148;
     if ((e = launch_pdl(k_attn_few<T, D>, ctas, kFewThreads, kFewSmem, s, a)) != cudaSuccess) return e;

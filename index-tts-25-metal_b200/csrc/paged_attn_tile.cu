@@ -641,7 +641,7 @@ cudaError_t launch(const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorM
                    cudaStream_t s) {
     constexpr size_t smem = sizeof(TileSmem<D>) + 1024;
     static_assert(smem <= 227 * 1024, "shared memory of a CTA");
-    cudaError_t e = cudaFuncSetAttribute(k_attn_tile<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+    cudaError_t e = allow_smem<k_attn_tile<T, D>>(smem);
     if (e != cudaSuccess) return e;
     if ((e = launch_pdl(k_attn_tile<T, D>, kTileCtas, kTileThreads, smem, s, mk, mv, mq, a, q_tokens)) != cudaSuccess) return e;
     return launch_pdl(k_join_rows<T, kTileRows, D>, dim3(kTileCtas, kTileRows / join_rows(D)), kJoinThreads, 0, s, a);

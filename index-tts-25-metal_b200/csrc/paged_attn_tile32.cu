@@ -507,7 +507,7 @@ template <int D>
 cudaError_t launch(const Attn& a, cudaStream_t s) {
     constexpr size_t smem = sizeof(Smem32<D>) + 1024;
     static_assert(smem <= 227 * 1024, "shared memory of a CTA");
-    cudaError_t e = cudaFuncSetAttribute(k_attn_tile32<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+    cudaError_t e = allow_smem<k_attn_tile32<D>>(smem);
     if (e != cudaSuccess) return e;
     if ((e = launch_pdl(k_attn_tile32<D>, kCtas32, kThreads32, smem, s, a)) != cudaSuccess) return e;
     return launch_pdl(k_join_rows<float, kRows32, D>, dim3(kCtas32, kRows32 / join_rows(D)), kJoinThreads, 0, s, a);

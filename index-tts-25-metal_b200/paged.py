@@ -10,6 +10,7 @@ returns at once; it can be captured into a CUDA graph.  Failures raise as in
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import torch
 
@@ -55,64 +56,96 @@ class Attention(C.Structure):
                 ("workspace_bytes", C.c_size_t)]
 
 
+# The structs are packed by hand below: a ctypes.Structure costs microseconds per
+# call.  Native alignment, so the layouts are those of the classes above.
+_PACK_TABLES = struct.Struct("iiiiqi11P").pack
+_PACK_APPEND = struct.Struct("PPiiiiii6q" "PPii4qP").pack
+_PACK_ATTENTION = struct.Struct("PPiiiiii6q" "PPii4q3PqiiifPN").pack
+
+_I32 = torch.int32
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+class _Entries:
+    """The library's entry points, looked up once."""
+    tables = append = attention = None
+    workspace = {}  # bytes by head_dim
+
+
+def _load():
+    lib = gpt.load_library()
+    _Entries.tables, _Entries.append, _Entries.attention = (lib.itts_paged_tables, lib.itts_paged_append,
+                                                            lib.itts_paged_attention)
+
+
 def _refuse(message: str):
     raise gpt.GptInvalidArgument(gpt.ERR_INVALID_ARGUMENT, message)
 
 
-def _run(entry, args, device: torch.device):
-    rc = entry(device.index, C.byref(args), torch._C._cuda_getCurrentRawStream(device.index))
-    if rc != gpt.OK:
-        gpt._raise(rc, gpt.load_library().itts_paged_last_error().decode())
+def _failed(rc: int):
+    gpt._raise(rc, gpt.load_library().itts_paged_last_error().decode())
 
 
-def _words(t, name: str, device, count: int):
-    """Address of a contiguous int32 vector of at least `count` entries."""
-    if t.dtype is not torch.int32 or t.device != device or t.dim() != 1 or t.shape[0] < count or \
-            (t.shape[0] > 1 and t.stride(0) != 1):
-        _refuse(f"{name} must be a contiguous int32 vector of {count} entries on {device}")
+def _device(t, name: str) -> int:
+    device = t.get_device()
+    if device < 0:
+        _refuse(f"{name} must be a CUDA tensor")
+    return device
+
+
+def _words(t, name: str, device: int, count: int) -> int:
+    """Address of a contiguous int32 tensor of at least `count` entries."""
+    if t.dtype is not _I32 or t.get_device() != device or t.numel() < count or not t.is_contiguous():
+        _refuse(f"{name} must be a contiguous int32 tensor of {count} entries on cuda:{device}")
     return t.data_ptr()
 
 
-def _table(table, requests: int, device):
-    if table.dtype is not torch.int32 or table.device != device or table.dim() != 2 or table.shape[0] < requests or \
-            (table.shape[1] > 1 and table.stride(1) != 1):
-        _refuse(f"table must be an int32 matrix of {requests} rows, contiguous columns, on {device}")
-    return table.data_ptr(), (table.stride(0) if table.shape[0] > 1 else table.shape[1]), table.shape[1]
+def _table(table, requests: int, device: int):
+    """Address, row stride and columns of a block table."""
+    if table.dtype is not _I32 or table.get_device() != device or table.dim() != 2:
+        _refuse(f"table must be an int32 matrix on cuda:{device}")
+    rows, columns = table.shape
+    if rows < requests:
+        _refuse(f"table must have {requests} rows")
+    if table.is_contiguous():
+        return table.data_ptr(), columns, columns
+    if columns > 1 and table.stride(1) != 1:
+        _refuse("table must have contiguous columns")
+    return table.data_ptr(), (table.stride(0) if rows > 1 else columns), columns
 
 
-def _cuda(t, name: str) -> torch.device:
-    if not t.is_cuda:
-        _refuse(f"{name} must be a CUDA tensor")
-    return t.device
-
-
-def _cache(k_cache, v_cache, device) -> Cache:
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+def _cache(k_cache, v_cache, device: int):
+    """The fields of an itts_paged_cache."""
+    kind = k_cache.dtype
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape:
         _refuse("k_cache and v_cache must be [blocks, block_size, heads, head_dim]")
-    if k_cache.dtype not in _TYPES or v_cache.dtype is not k_cache.dtype:
+    if kind not in _TYPES or v_cache.dtype is not kind:
         _refuse("paged cache type is f32, f16 or bf16")
-    if k_cache.device != device or v_cache.device != device:
-        _refuse(f"k_cache and v_cache must be on {device}")
+    if k_cache.get_device() != device or v_cache.get_device() != device:
+        _refuse(f"k_cache and v_cache must be on cuda:{device}")
     kb, kt, kh, kd = k_cache.stride()
     vb, vt, vh, vd = v_cache.stride()
     if kd != 1 or vd != 1:
         _refuse("the head dimension of a paged cache must be contiguous")
-    blocks, size, heads, dim = k_cache.shape
+    blocks, size, heads, dim = shape
     # the stride of a dimension of one is never used, and torch may give it any value
     if blocks == 1:
         kb = vb = 0
     if heads == 1:
         kh = vh = 0
-    return Cache(k_cache.data_ptr(), v_cache.data_ptr(), _TYPES[k_cache.dtype], blocks, size, heads, dim, 0, kb, kt,
-                 kh, vb, vt, vh)
+    return k_cache.data_ptr(), v_cache.data_ptr(), _TYPES[kind], blocks, size, heads, dim, 0, kb, kt, kh, vb, vt, vh
 
 
-def _rows(t, name: str, dtype, heads, dim: int, device):
-    """Address and row / head strides of a [rows, heads, head_dim] tensor."""
-    if t.dim() != 3 or t.shape[2] != dim or (heads and t.shape[1] != heads) or t.dtype is not dtype or \
-            t.device != device or t.stride(2) != 1:
-        _refuse(f"{name} must be [rows, heads, {dim}] of {dtype} with a contiguous last dimension on {device}")
-    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0
+def _rows(t, name: str, dtype, dim: int, device: int):
+    """Address, rows, heads and row / head strides of a [rows, heads, head_dim] tensor."""
+    if t.dim() != 3 or t.dtype is not dtype or t.get_device() != device:
+        _refuse(f"{name} must be [rows, heads, head_dim] of {dtype} on cuda:{device}")
+    rows, heads, last = t.shape
+    row, head, one = t.stride()
+    if last != dim or one != 1:
+        _refuse(f"{name} must have a contiguous last dimension of {dim}")
+    return t.data_ptr(), rows, heads, (row if rows > 1 else 0), (head if heads > 1 else 0)
 
 
 def tables(cached, fresh, table, free_list, free_count, block_size: int, *, lens, q_start, positions, slots, status,
@@ -123,38 +156,48 @@ def tables(cached, fresh, table, free_list, free_count, block_size: int, *, lens
     [blocks] (written); free_count [1].  Outputs: lens [requests], q_start
     [requests + 1], positions and slots [rows], status [1] and free_out [1]
     (free_count itself if not given).  ``lens`` may be ``cached``."""
-    device = _cuda(cached, "cached")
-    n, rows = fresh.shape[0] if fresh.dim() == 1 else -1, slots.shape[0] if slots.dim() == 1 else -1
+    device = _device(cached, "cached")
+    n, rows = fresh.numel(), slots.numel()
     address, stride, columns = _table(table, n, device)
     count = _words(free_count, "free_count", device, 1)
-    blocks = free_list.shape[0] if free_list.dim() == 1 else -1
-    a = Tables(n, block_size, blocks, columns, stride, rows, _words(cached, "cached", device, n),
-               _words(fresh, "fresh", device, n), address, _words(free_list, "free_list", device, 1), count,
-               count if free_out is None else _words(free_out, "free_out", device, 1),
-               _words(lens, "lens", device, n), _words(q_start, "q_start", device, n + 1),
-               _words(positions, "positions", device, rows), _words(slots, "slots", device, rows),
-               _words(status, "status", device, 1))
-    _run(gpt.load_library().itts_paged_tables, a, device)
+    try:
+        args = _PACK_TABLES(n, block_size, free_list.numel(), columns, stride, rows, _words(cached, "cached", device, n),
+                            _words(fresh, "fresh", device, n), address, _words(free_list, "free_list", device, 1), count,
+                            count if free_out is None else _words(free_out, "free_out", device, 1),
+                            _words(lens, "lens", device, n), _words(q_start, "q_start", device, n + 1),
+                            _words(positions, "positions", device, rows), _words(slots, "slots", device, rows),
+                            _words(status, "status", device, 1))
+    except struct.error as e:
+        _refuse(f"argument out of range: {e}")
+    if _Entries.tables is None:
+        _load()
+    rc = _Entries.tables(device, args, _stream(device))
+    if rc:
+        _failed(rc)
 
 
 def append(k, v, k_cache, v_cache, slots):
     """Writes rows k, v [rows, heads, head_dim] (the caches' type, or float32)
     into the caches [blocks, block_size, heads, head_dim] at ``slots`` [rows];
     rows with a slot outside the cache are left out (itts_paged_append)."""
-    device = _cuda(k, "k")
-    c = _cache(k_cache, v_cache, device)
-    if k.dtype not in _TYPES:
+    device = _device(k, "k")
+    cache = _cache(k_cache, v_cache, device)
+    kind = k.dtype
+    if kind not in _TYPES:
         _refuse("source type is the cache's type or f32")
-    rows = k.shape[0]
-    kp, kr, kh = _rows(k, "k", k.dtype, c.heads, c.head_dim, device)
-    vp, vr, vh = _rows(v, "v", k.dtype, c.heads, c.head_dim, device)
-    if v.shape[0] != rows:
-        _refuse("k and v must have the same rows")
-    a = Append(c, kp, vp, _TYPES[k.dtype], rows, kr, kh, vr, vh, _words(slots, "slots", device, rows))
-    _run(gpt.load_library().itts_paged_append, a, device)
-
-
-_WORKSPACE: dict = {}  # bytes by head_dim
+    kp, rows, heads, kr, kh = _rows(k, "k", kind, cache[6], device)
+    vp, vrows, vheads, vr, vh = _rows(v, "v", kind, cache[6], device)
+    if vrows != rows or heads != cache[5] or vheads != cache[5]:
+        _refuse("k and v must have the same rows and the caches' heads")
+    try:
+        args = _PACK_APPEND(*cache, kp, vp, _TYPES[kind], rows, kr, kh, vr, vh, _words(slots, "slots", device, rows))
+    except struct.error as e:
+        _refuse(f"argument out of range: {e}")
+    if _Entries.append is None:
+        _load()
+    rc = _Entries.append(device, args, _stream(device))
+    if rc:
+        _failed(rc)
 
 
 def attention(q, k_cache, v_cache, table, lens, q_start, max_fresh: int, scale: float | None = None, out=None,
@@ -167,28 +210,36 @@ def attention(q, k_cache, v_cache, table, lens, q_start, max_fresh: int, scale: 
     ``workspace``: a uint8 CUDA tensor of ``workspace_bytes(head_dim)`` that no
     other call uses at the same time; by default one is taken from torch's
     allocator for the call."""
-    device = _cuda(q, "q")
-    c = _cache(k_cache, v_cache, device)
-    qp, qr, qh = _rows(q, "q", k_cache.dtype, None, c.head_dim, device)
-    rows, heads = q.shape[0], q.shape[1]
+    device = _device(q, "q")
+    cache = _cache(k_cache, v_cache, device)
+    kind, dim = k_cache.dtype, cache[6]
+    qp, rows, heads, qr, qh = _rows(q, "q", kind, dim, device)
     if out is None:
-        out = torch.empty((rows, heads, c.head_dim), dtype=q.dtype, device=device)
-    elif out.shape[0] != rows:
+        out = torch.empty((rows, heads, dim), dtype=kind, device=q.device)
+    op, orows, oheads, orow, oh = _rows(out, "out", kind, dim, device)
+    if orows != rows or oheads != heads:
         _refuse("out must have q's shape")
-    op, orow, oh = _rows(out, "out", k_cache.dtype, heads, c.head_dim, device)
-    requests = lens.shape[0] if lens.dim() == 1 else -1
+    requests = lens.numel()
     address, stride, columns = _table(table, requests, device)
-    need = _WORKSPACE.get(c.head_dim)
-    if need is None:
-        need = _WORKSPACE[c.head_dim] = workspace_bytes(c.head_dim)
     if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    elif workspace.device != device or workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
-        _refuse(f"workspace must be a contiguous uint8 tensor on {device}")
-    a = Attention(c, qp, op, heads, rows, qr, qh, orow, oh, _words(q_start, "q_start", device, requests + 1),
-                  _words(lens, "lens", device, requests), address, stride, requests, columns, max_fresh,
-                  c.head_dim ** -0.5 if scale is None else scale, workspace.data_ptr(), workspace.numel())
-    _run(gpt.load_library().itts_paged_attention, a, device)
+        need = _Entries.workspace.get(dim)
+        if need is None:
+            need = _Entries.workspace[dim] = workspace_bytes(dim)
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    elif workspace.get_device() != device or workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
+        _refuse(f"workspace must be a contiguous uint8 tensor on cuda:{device}")
+    try:
+        args = _PACK_ATTENTION(*cache, qp, op, heads, rows, qr, qh, orow, oh,
+                               _words(q_start, "q_start", device, requests + 1), _words(lens, "lens", device, requests),
+                               address, stride, requests, columns, max_fresh, dim ** -0.5 if scale is None else scale,
+                               workspace.data_ptr(), workspace.numel())
+    except struct.error as e:
+        _refuse(f"argument out of range: {e}")
+    if _Entries.attention is None:
+        _load()
+    rc = _Entries.attention(device, args, _stream(device))
+    if rc:
+        _failed(rc)
     return out
 
 

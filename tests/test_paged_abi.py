@@ -161,6 +161,23 @@ def test_no_rows_is_no_work(lib, gpt_mod, paged):
     assert lib.itts_paged_attention(0, C.byref(b), None) == gpt_mod.OK
 
 
+def test_packed_arguments_match_the_structs(paged):
+    """paged.py packs the argument structs by hand: byte for byte what the ctypes classes hold."""
+    for pack, kind in ((paged._PACK_TABLES, paged.Tables), (paged._PACK_APPEND, paged.Append),
+                       (paged._PACK_ATTENTION, paged.Attention)):
+        def flat(cls):
+            for _, t in cls._fields_:
+                yield from flat(t) if hasattr(t, "_fields_") else [t]
+
+        values = [0.5 if t is C.c_float else 1000003 * (i + 1) for i, t in enumerate(flat(kind))]
+        it = iter(values)
+
+        def build(cls):
+            return cls(*[build(t) if hasattr(t, "_fields_") else next(it) for _, t in cls._fields_])
+
+        assert bytes(build(kind)) == pack(*values)
+
+
 def test_python_binding_refuses_host_tensors(gpt_mod, paged):
     import torch
     i = torch.zeros(4, dtype=torch.int32)
