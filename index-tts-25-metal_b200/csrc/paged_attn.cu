@@ -9,7 +9,7 @@ namespace itts {
 namespace paged {
 
 size_t few_workspace_floats(int head_dim);
-cudaError_t launch_few(const Attn& a, cudaStream_t s);
+cudaError_t launch_few(const Attn& a, long long rows, cudaStream_t s);
 size_t tile_workspace_floats(int head_dim);
 cudaError_t launch_tile(const Attn& a, cudaStream_t s);
 size_t tile32_workspace_floats(int head_dim);
@@ -42,6 +42,10 @@ cudaError_t launch_attention(const itts_paged_attention_args& p, cudaStream_t s)
     a.rows = p.rows;
     a.requests = p.requests;
     a.group = p.q_heads / p.cache.heads;
+    int bits = 0;
+    while ((1 << bits) < a.group) ++bits;
+    a.group_shift = 30 + bits;
+    a.group_mul = uint32_t(((uint64_t(1) << a.group_shift) + a.group - 1) / a.group);
     while ((1 << a.shift) < p.cache.block_size) ++a.shift;
     a.cap = p.max_blocks << a.shift;
     a.scale2 = std::fmax(std::fabs(p.scale) * kLog2e, 1e-30f);
@@ -53,7 +57,7 @@ cudaError_t launch_attention(const itts_paged_attention_args& p, cudaStream_t s)
         const cudaError_t e = launch_tile(a, s);
         if (e != cudaErrorNotSupported) return e;
     }
-    return launch_few(a, s);
+    return launch_few(a, (long long)p.max_fresh * a.group, s);
 }
 
 }  // namespace paged

@@ -55,11 +55,17 @@ struct Attn {
     long long table_stride;
     int rows, requests, group, shift;  // group = q_heads / heads, shift = log2(block_size)
     int cap;                           // keys that the table's columns can name
+    uint32_t group_mul;                // r / group = r * group_mul >> group_shift for r < 2^30
+    int group_shift;
     float scale2;                      // |scale| log2(e), at least 1e-30: a masked -inf stays -inf
     float sign;                        // of the scale, taken into q
     float* part;                       // partial sums
     int4* rec;                         // per CTA: {CTAs of the item that begins here, first row, kv head, rows}
 };
+
+__device__ __forceinline__ int over_group(const Attn& a, int r) {
+    return int((unsigned long long)(unsigned)r * a.group_mul >> a.group_shift);
+}
 
 // A request's rows and keys.
 struct Request {
@@ -72,7 +78,7 @@ struct Request {
         rows = tokens * a.group;  // the host has checked that a.rows * group <= 2^30
     }
     // Position of the token of row r.
-    __device__ __forceinline__ int pos(const Attn& a, int r) const { return len - tokens + r / a.group; }
+    __device__ __forceinline__ int pos(const Attn& a, int r) const { return len - tokens + over_group(a, r); }
     // Keys that some row of tile t sees.
     template <int RT>
     __device__ __forceinline__ int keys(const Attn& a, int t) const {
@@ -98,25 +104,38 @@ struct Share {
     int ctas;                 // that have a share: every one of them at least one unit
     int b;                    // request of u0
     long long base;           // units before that request
+    Request r;                // that request
 };
 
 template <int kThreadsT>
 struct PlanSmem {
-    long long warp_sum[kThreadsT / 32 + 1];
+    long long warp_sum[kThreadsT / 32];
     Share share;
 };
 
-// Called by all threads of the CTA.  `ctas` is what the launch may use; with
-// few units the last CTAs get none.
+// Called by all threads of the CTA.  Returns the units of its share (0: none),
+// which is then in sm.share.  `scratch`: an int per request in shared memory,
+// used where there are more requests than threads.
 template <int RT, int KU, int kThreadsT>
-__device__ Share plan(const Attn& a, int cta, int ctas, PlanSmem<kThreadsT>& sm) {
+__device__ int plan(const Attn& a, int cta, int ctas, PlanSmem<kThreadsT>& sm, int* scratch) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int per = (a.requests + kThreadsT - 1) / kThreadsT, b0 = tid * per;
+    const int per = (a.requests + kThreadsT - 1) / kThreadsT, b0 = tid * per, b1 = min(a.requests, b0 + per);
     long long mine = 0;
-    for (int b = b0; b < min(a.requests, b0 + per); ++b) {
-        Request r;
-        r.load(a, b);
-        mine += r.total<RT, KU>(a);
+    Request r{};
+    if (per == 1) {
+        if (b0 < b1) {
+            r.load(a, b0);
+            mine = r.total<RT, KU>(a);
+        }
+    } else {  // coalesced loads, several in flight; then each thread adds up its requests in a row
+#pragma unroll 4
+        for (int b = tid; b < a.requests; b += kThreadsT) {
+            Request x;
+            x.load(a, b);
+            scratch[b] = int(x.total<RT, KU>(a));
+        }
+        __syncthreads();
+        for (int b = b0; b < b1; ++b) mine += scratch[b];
     }
     mine *= a.c.heads;
     long long inc = mine;
@@ -133,28 +152,23 @@ __device__ Share plan(const Attn& a, int cta, int ctas, PlanSmem<kThreadsT>& sm)
         if (w < warp) before += sm.warp_sum[w];
         all += sm.warp_sum[w];
     }
-    Share s;
+    Share s{};
     s.units = all;
     s.ctas = int(min((long long)ctas, all));
     s.u0 = cta < s.ctas ? all * cta / s.ctas : all;
     s.u1 = cta < s.ctas ? all * (cta + 1) / s.ctas : all;
-    s.b = 0;
-    s.base = 0;
-    if (tid == 0) sm.share = s;
-    __syncthreads();
-    if (mine > 0 && before <= s.u0 && s.u0 < before + mine) {  // one thread holds the request of u0
+    if (before <= s.u0 && s.u0 < before + mine) {  // one thread holds the request of u0
         s.base = before;
-        for (s.b = b0;; ++s.b) {
-            Request r;
+        s.b = b0;
+        if (per > 1) {
+            while (s.u0 >= s.base + (long long)scratch[s.b] * a.c.heads) s.base += (long long)scratch[s.b++] * a.c.heads;
             r.load(a, s.b);
-            const long long n = r.total<RT, KU>(a) * a.c.heads;
-            if (s.u0 < s.base + n) break;
-            s.base += n;
         }
+        s.r = r;
         sm.share = s;
     }
     __syncthreads();
-    return sm.share;
+    return int(s.u1 - s.u0);
 }
 
 // Walks the items of a share, unit by unit.
@@ -165,7 +179,7 @@ struct Walk {
     int k, nk;        // unit of the item, units of the item
     __device__ __forceinline__ void start(const Attn& a, const Share& s) {
         b = s.b;
-        r.load(a, b);
+        r = s.r;
         t = 0;
         long long left = s.u0 - s.base;
         for (;; ++t) {
@@ -200,10 +214,11 @@ __device__ __forceinline__ int cta_of(const Share& s, long long u) {
 }
 
 // Partial sums of an item: RT rows of D unnormalised outputs, then RT pairs
-// (maximum in units of log2, sum).
+// (maximum in units of log2, sum); slots are multiples of 128 bytes, so that the
+// rows keep the alignment of their 16-byte accesses whatever RT is.
 template <int RT, int D>
 __host__ __device__ constexpr size_t part_floats() {
-    return size_t(RT) * (D + 2);
+    return (size_t(RT) * (D + 2) + 31) / 32 * 32;
 }
 template <int RT, int D>
 __device__ __forceinline__ float* part_slot(const Attn& a, int cta, int which) {
@@ -235,7 +250,7 @@ __device__ __forceinline__ void store4<__nv_bfloat16>(__nv_bfloat16* p, float4 v
 // request that starts at `start`) goes.
 template <class T>
 __device__ __forceinline__ T* out_row(const Attn& a, int start, int first, int row, int kvh) {
-    const int r = first + row, tok = r / a.group, g = r - tok * a.group;
+    const int r = first + row, tok = over_group(a, r), g = r - tok * a.group;
     return static_cast<T*>(a.out) + (long long)(start + tok) * a.o_row + (long long)(kvh * a.group + g) * a.o_head;
 }
 

@@ -245,15 +245,17 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         sm.abort = 0;
     }
     pdl_wait();
-    const Share sh = plan<kTileRows, kUnitKeys, kTileThreads>(a, blockIdx.x, gridDim.x, sm.plan);
+    const int units = plan<kTileRows, kUnitKeys, kTileThreads>(a, blockIdx.x, gridDim.x, sm.plan, reinterpret_cast<int*>(sm.kv));
+    const Share& sh = sm.plan.share;
     if (threadIdx.x == 0) put_record(a, blockIdx.x, 0, 0, 0, 0, 0);
-    const int n = uniform(int(sh.u1 - sh.u0));
+    const int n = uniform(units);
     if (n == 0) return;
     if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sm.tmem))
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the plan's scratch lies where TMA writes next
     tc_before();
     __syncthreads();
     tc_after();
@@ -436,7 +438,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
                         for (int hf = 0; hf < kHalves; ++hf)
                             tma_rows(smem_u32(sm.q[t]) + hf * kHalfBytes, &map_q, 64 * hf, g.kvh * a.group,
-                                     g.start + row0 / a.group, &sm.q_full[t]);
+                                     g.start + over_group(a, row0), &sm.q_full[t]);
                     }
                 } else {
                     const uint32_t flip = a.sign < 0.f ? 0x80008000u : 0u;
@@ -446,7 +448,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         const int r = y / kChunks, ch = y % kChunks;
                         uint4 v = make_uint4(0, 0, 0, 0);
                         if (128 * t + r < g.rows) {
-                            const int tok = (row0 + r) / a.group, hd = (row0 + r) - tok * a.group;
+                            const int tok = over_group(a, row0 + r), hd = (row0 + r) - tok * a.group;
                             v = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) +
                                                                      (long long)(g.start + tok) * a.q_row +
                                                                      (long long)(g.kvh * a.group + hd) * a.q_head) + ch);
@@ -483,7 +485,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             const Segment& g = sm.seg[x % kSegments];
             const int units = g.tu[t];
             int seen = 0;  // keys of the unit that the row sees
-            if (row < g.rows) seen = min(max(g.pos + (g.first + row) / a.group + 1, 0), a.cap) - g.k0 * kUnitKeys;
+            if (row < g.rows) seen = min(max(g.pos + over_group(a, g.first + row) + 1, 0), a.cap) - g.k0 * kUnitKeys;
             else seen = -g.k0 * kUnitKeys;
             float m = -INFINITY, l = 0.f;
             for (int j = 0; j < units; ++j, seen -= kUnitKeys) {

@@ -23,8 +23,8 @@
 //         unit ahead, split them and write the words to shared memory, two stages
 //         of 48 KB each for K and V.  What is behind the item's keys or in a bad
 //         block is not read: zeros.
-//   4     warp 16 issues the products, warp 17 walks the items and publishes
-//         their extents in shared memory.
+//   4     warp 16 issues the products; warps 17 and 18 walk the items and publish
+//         in shared memory their extents and where their units' keys lie.
 // Tensor memory: Q (three words), two buffers of scores / P, O.  With two score
 // buffers Q K^T of unit j + 2 follows P V of unit j in the queue, so the tensor
 // core has work while the softmax of j + 1 runs, and O is drained meanwhile.
@@ -51,6 +51,13 @@ struct Segment32 {
     int parts;               // 0: begins and ends here; 1: goes on from another share; n > 1: begins here, n shares
 };
 
+// Where the keys of a unit lie.
+struct Unit32 {
+    int ids[kUnit32 / 16];  // block of 16 keys, -1: none that the table names
+    int keys, tok, kvh;     // keys left in the item, token of the first in its block, kv head
+};
+constexpr int kUnits32 = 8;
+
 template <int D>
 struct alignas(1024) Smem32 {
     static constexpr int kWord = kUnit32 * D * 2;  // one word of a K or V tile
@@ -58,7 +65,8 @@ struct alignas(1024) Smem32 {
     unsigned char v[2][3][kWord];
     unsigned long long k_full[2], k_empty[2], v_full[2], v_empty[2], s_ready[2], p_ready[2], f_ready[4];
     unsigned long long q_full, o_done, o_free, done;
-    unsigned long long seg_full[kSegments32], seg_empty[kSegments32];
+    unsigned long long seg_full[kSegments32], seg_empty[kSegments32], unit_full[kUnits32], unit_empty[kUnits32];
+    Unit32 unit[kUnits32];
     float2 ml[4][kRows32];  // of unit j at j % 4: running maximum and sum,
     float f[4][kRows32];    // and what they rescale the output by
     Segment32 seg[kSegments32];
@@ -164,6 +172,10 @@ __global__ void __launch_bounds__(kThreads32, 1) k_attn_tile32(const __grid_cons
             mbar_init(&sm.seg_full[s], 1);
             mbar_init(&sm.seg_empty[s], 9);  // softmax and output warps, products
         }
+        for (int s = 0; s < kUnits32; ++s) {
+            mbar_init(&sm.unit_full[s], 1);
+            mbar_init(&sm.unit_empty[s], 8);
+        }
         mbar_init(&sm.q_full, 4);
         mbar_init(&sm.o_done, 1);
         mbar_init(&sm.o_free, 4);
@@ -172,9 +184,10 @@ __global__ void __launch_bounds__(kThreads32, 1) k_attn_tile32(const __grid_cons
         sm.abort = 0;
     }
     pdl_wait();
-    const Share sh = plan<kRows32, kUnit32, kThreads32>(a, blockIdx.x, gridDim.x, sm.plan);
+    const int units = plan<kRows32, kUnit32, kThreads32>(a, blockIdx.x, gridDim.x, sm.plan, reinterpret_cast<int*>(sm.k));
+    const Share& sh = sm.plan.share;
     if (threadIdx.x == 0) put_record(a, blockIdx.x, 0, 0, 0, 0, 0);
-    const int n = uniform(int(sh.u1 - sh.u0));
+    const int n = uniform(units);
     if (n == 0) return;
     if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sm.tmem))
@@ -199,7 +212,7 @@ __global__ void __launch_bounds__(kThreads32, 1) k_attn_tile32(const __grid_cons
             int seen = -g.k0 * kUnit32;  // keys of the unit that the row sees
             const bool live = row < g.rows;
             {
-                const int r = g.first + row, tok = r / a.group;
+                const int r = g.first + row, tok = over_group(a, r);
                 if (live) seen += min(max(g.pos + tok + 1, 0), a.cap);
                 // every product with the Q before is done: the last unit's scores were read
                 const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(a.q) +
@@ -316,12 +329,12 @@ __global__ void __launch_bounds__(kThreads32, 1) k_attn_tile32(const __grid_cons
                 if (!ok) break;
                 tc_after();
 #pragma unroll
-                for (int c = 0; c < D / 16; ++c) {
-                    uint32_t v[16];
-                    tmem_ld16(lanes + kO + 16u * c, v);
+                for (int c = 0; c < D / 8; ++c) {
+                    uint32_t v[8];
+                    tmem_ld8(lanes + kO + 8u * c, v);
                     tc_wait_ld(v);
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) o[16 * c + e] = fmaf(o[16 * c + e], f, __uint_as_float(v[e]));
+                    for (int e = 0; e < 8; ++e) o[8 * c + e] = fmaf(o[8 * c + e], f, __uint_as_float(v[e]));
                 }
                 tc_before();
                 __syncwarp();
@@ -354,22 +367,16 @@ __global__ void __launch_bounds__(kThreads32, 1) k_attn_tile32(const __grid_cons
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsSplit));
         constexpr int kLanes = D / 4, kPer = 32 / kLanes, kLoads = 8 / kPer;  // lanes of a key, keys at once, loads
         const int c = warp - 8, key = 8 * c + lane / kLanes, d4 = lane % kLanes;
-        Walk32 w;
-        w.start(a, sh);
-        const auto where = [&] {  // block of this warp's keys in the walk's unit
-            const long long page = ((long long)w.k * kUnit32 + 8 * c) >> a.shift;
-            return page < (a.cap >> a.shift) && (page << a.shift) < w.r.len ? __ldcg(a.table + w.b * a.table_stride + page) : -1;
-        };
         float4 kr[kLoads], vr[kLoads];
-        int keys = w.r.keys<kRows32>(a, w.t), id = where();
-        const auto load = [&](float4 (&y)[kLoads], const void* base, long long bs, long long ts, long long hs) {
-            const bool named = (unsigned)id < (unsigned)a.c.blocks;
-            const int key0 = w.k * kUnit32 + key, tok = key0 & ((1 << a.shift) - 1);
-            const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(base) + (named ? id : 0) * bs +
-                                                              tok * ts + w.h * hs) + d4;
+        const auto load = [&](float4 (&y)[kLoads], const Unit32& w, const void* base, long long bs, long long ts, long long hs) {
+            const int id = w.ids[c >> 1], keys = id < 0 ? 0 : w.keys - key, tok = (w.tok + key) & ((1 << a.shift) - 1);
+            const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(base) + max(id, 0) * bs + tok * ts +
+                                                              w.kvh * hs) + d4;
 #pragma unroll
-            for (int e = 0; e < kLoads; ++e)
-                y[e] = named && key0 + e * kPer < keys ? __ldg(p + e * kPer * (ts / 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int e = 0; e < kLoads; ++e) {
+                y[e] = e * kPer < keys ? __ldg(p) : make_float4(0.f, 0.f, 0.f, 0.f);
+                p += kPer * (ts / 4);
+            }
         };
         const auto store = [&](const float4 (&y)[kLoads], unsigned char (*tile)[Smem::kWord]) {
 #pragma unroll
@@ -386,31 +393,34 @@ __global__ void __launch_bounds__(kThreads32, 1) k_attn_tile32(const __grid_cons
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
         };
-        load(kr, a.c.k, a.c.k_block_stride, a.c.k_token_stride, a.c.k_head_stride);
-        load(vr, a.c.v, a.c.v_block_stride, a.c.v_token_stride, a.c.v_head_stride);
-        bool ok = true;
-        for (int i = 0; i < n; ++i) {
+        // the unit's K and V are in registers when its turn comes, the next unit's loads follow them
+        bool ok = uniform(mbar_wait(&sm.unit_full[0], 0u, &sm.abort));
+        if (ok) {
+            load(kr, sm.unit[0], a.c.k, a.c.k_block_stride, a.c.k_token_stride, a.c.k_head_stride);
+            load(vr, sm.unit[0], a.c.v, a.c.v_block_stride, a.c.v_token_stride, a.c.v_head_stride);
+        }
+        for (int i = 0; i < n && ok; ++i) {
             const int s = i & 1;
-            const bool bad = (unsigned)id >= (unsigned)a.c.blocks;
             const bool more = i + 1 < n;
+            const Unit32& next = sm.unit[(i + 1) % kUnits32];
             if (i >= 2) ok = uniform(mbar_wait(&sm.k_empty[s], uint32_t((i >> 1) + 1) & 1u, &sm.abort));
             if (!ok) break;
-            if (lane == 0 && (c & 1) == 0) *reinterpret_cast<volatile unsigned*>(&sm.bad[i & 3][c >> 1]) = bad;
+            if (lane == 0 && (c & 1) == 0)
+                *reinterpret_cast<volatile unsigned*>(&sm.bad[i & 3][c >> 1]) = sm.unit[i % kUnits32].ids[c >> 1] < 0;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.unit_empty[i % kUnits32]);
             store(kr, sm.k[s]);
             if (lane == 0) mbar_arrive(&sm.k_full[s]);
             if (more) {
-                if (++w.k == w.nk) {
-                    w.next(a);
-                    keys = w.r.keys<kRows32>(a, w.t);
-                }
-                id = where();
-                load(kr, a.c.k, a.c.k_block_stride, a.c.k_token_stride, a.c.k_head_stride);
+                ok = uniform(mbar_wait(&sm.unit_full[(i + 1) % kUnits32], uint32_t((i + 1) / kUnits32) & 1u, &sm.abort));
+                if (!ok) break;
+                load(kr, next, a.c.k, a.c.k_block_stride, a.c.k_token_stride, a.c.k_head_stride);
             }
             if (i >= 2) ok = uniform(mbar_wait(&sm.v_empty[s], uint32_t((i >> 1) + 1) & 1u, &sm.abort));
             if (!ok) break;
             store(vr, sm.v[s]);
             if (lane == 0) mbar_arrive(&sm.v_full[s]);
-            if (more) load(vr, a.c.v, a.c.v_block_stride, a.c.v_token_stride, a.c.v_head_stride);
+            if (more) load(vr, next, a.c.v, a.c.v_block_stride, a.c.v_token_stride, a.c.v_head_stride);
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
@@ -490,6 +500,32 @@ __global__ void __launch_bounds__(kThreads32, 1) k_attn_tile32(const __grid_cons
                 if (i < n) {
                     w.k += g.n - 1;  // to the item's last unit, and over it
                     w.next(a);
+                }
+            }
+        } else if (warp == 18) {
+            // ---- units: lane = 16 keys
+            Walk32 w;
+            w.start(a, sh);
+            int keys = w.r.keys<kRows32>(a, w.t);
+            bool ok = true;
+            for (int i = 0; i < n; ++i) {
+                const int x = i % kUnits32;
+                const int key0 = w.k * kUnit32 + 16 * lane, page = key0 >> a.shift;
+                int id = -1;
+                if (lane < kUnit32 / 16 && key0 < keys) id = __ldcg(a.table + w.b * a.table_stride + page);
+                if (i >= kUnits32) ok = uniform(mbar_wait(&sm.unit_empty[x], uint32_t(i / kUnits32 + 1) & 1u, &sm.abort));
+                if (!ok) break;
+                if (lane < kUnit32 / 16) sm.unit[x].ids[lane] = (unsigned)id < (unsigned)a.c.blocks ? id : -1;
+                if (lane == 0) {
+                    sm.unit[x].keys = keys - w.k * kUnit32;
+                    sm.unit[x].tok = (w.k * kUnit32) & ((1 << a.shift) - 1);
+                    sm.unit[x].kvh = w.h;
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.unit_full[x]);
+                if (i + 1 < n && ++w.k == w.nk) {
+                    w.next(a);
+                    keys = w.r.keys<kRows32>(a, w.t);
                 }
             }
         }
