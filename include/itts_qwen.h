@@ -50,10 +50,23 @@ int itts_qwen_step(itts_qwen_ctx* ctx, uint32_t id, float* logits);
  * ids go to out[0 .. *n_out) (out_cap >= maximum). */
 int itts_qwen_generate(itts_qwen_ctx* ctx, const uint32_t* ids, size_t n, uint32_t maximum, uint32_t* out,
                        size_t out_cap, uint32_t* n_out);
+/* generate for n independent prompts at once: prompt i is ids[i][0 .. n_ids[i]),
+ * its ids go to out[i * maximum ..), their number to n_out[i], and stopped[i]
+ * says whether the last one is EOS (a run of `maximum` ids without EOS is no
+ * failure here).  Every prompt is checked as generate checks it before any runs.
+ * No counterpart in the reference, which has one sequence per decoder.
+ *
+ * Up to 16 prompts are in flight, a finished one's place goes to the next.  Their
+ * keys and values share one paged cache (itts_paged.h); a step takes up to 1024
+ * rows: one for each prompt that is generating, chunks of the others.  The
+ * sequence of prefill / step / generate is left as it was. */
+int itts_qwen_generate_batch(itts_qwen_ctx* ctx, size_t n, const uint32_t* const* ids, const size_t* n_ids,
+                             uint32_t maximum, uint32_t* out, uint32_t* n_out, int32_t* stopped);
 uint32_t itts_qwen_cached_tokens(const itts_qwen_ctx* ctx);
 
 /* Device time of the last prefill / generate call (CUDA events on the
- * context's stream): the prompt pass, then the token steps. */
+ * context's stream): the prompt pass, then the token steps.  generate_batch: all
+ * its steps, and the prompt tokens of all prompts. */
 typedef struct itts_qwen_timing {
     float prefill_ms;
     float decode_ms;

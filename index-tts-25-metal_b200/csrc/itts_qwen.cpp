@@ -17,6 +17,7 @@
 #include <string>
 #include <vector>
 
+#include "itts_paged.h"
 #include "mit2_bundle.hpp"
 #include "qwen.hpp"
 
@@ -55,6 +56,23 @@ enum Mat : int { kMatQkv = 0, kMatO = 1, kMatGu = 2, kMatDown = 3 };
 constexpr int kMatRows[4] = {q::kQkv, q::kDim, 2 * q::kFfn, q::kDim};
 constexpr int kMatCols[4] = {q::kDim, q::kQDim, q::kDim, q::kFfn};
 
+// Device and pinned buffers of generate_batch, made by its first call.
+struct Batch {
+    float* kv = nullptr;  // [layer][K | V][blocks][kBlock][8][128], grown as calls need it
+    int32_t blocks = 0;
+    int32_t *lens = nullptr, *fresh = nullptr, *table = nullptr, *free_list = nullptr, *count = nullptr;
+    int32_t *q_start = nullptr, *positions = nullptr, *slots = nullptr, *status = nullptr;
+    q::State* st = nullptr;  // [kBatch]
+    uint32_t* out = nullptr; // [kBatch][kMaxGenerate]
+    void* workspace = nullptr;
+    struct Host {            // pinned
+        uint32_t ids[q::kStepRows];
+        int32_t fresh[q::kBatch];
+        int32_t status;
+        q::State st[q::kBatch];
+    }* h = nullptr;
+};
+
 }  // namespace
 
 struct itts_qwen_ctx {
@@ -76,6 +94,7 @@ struct itts_qwen_ctx {
     cudaEvent_t ev[3] = {nullptr, nullptr, nullptr};
     uint32_t cached = 0;
     itts_qwen_timing timing{};
+    Batch batch;
 
     ~itts_qwen_ctx() {
         cudaSetDevice(device);
@@ -83,6 +102,9 @@ struct itts_qwen_ctx {
         if (exec) cudaGraphExecDestroy(exec);
         if (graph) cudaGraphDestroy(graph);
         for (void* p : allocs) cudaFree(p);
+        if (batch.kv) cudaFree(batch.kv);
+        if (batch.free_list) cudaFree(batch.free_list);
+        if (batch.h) cudaFreeHost(batch.h);
         if (h_state) cudaFreeHost(h_state);
         for (cudaEvent_t e : ev)
             if (e) cudaEventDestroy(e);
@@ -245,6 +267,15 @@ void gemm(itts_qwen_ctx* c, int layer, int m, const itts::TmaMap* a, int epi, co
     qck(itts::tma_gemm(g, c->stream), "prompt GEMM");
 }
 
+void activation_maps(itts_qwen_ctx* c, int T) {
+    if (c->amap_rows == T) return;
+    const q::Buffers& b = c->b;
+    const float* base[6] = {b.x_hi, b.x_lo, b.att_hi, b.att_lo, b.gu_hi, b.gu_lo};
+    const int cols[6] = {q::kDim, q::kDim, q::kQDim, q::kQDim, q::kFfn, q::kFfn};
+    for (int i = 0; i < 6; ++i) qck(itts::tma_make_map(&c->amap[i], base[i], T, cols[i]), "tensor map");
+    c->amap_rows = T;
+}
+
 // The prompt pass (qwen.cpp:24-43 with t = n, offset 0): logits of the last
 // position and the argmax into the State (out[0]).
 void run_prompt(itts_qwen_ctx* c, const uint32_t* ids, size_t n, uint32_t max_out) {
@@ -252,12 +283,7 @@ void run_prompt(itts_qwen_ctx* c, const uint32_t* ids, size_t n, uint32_t max_ou
         if (ids[i] >= uint32_t(q::kVocab)) invalid("Invalid Qwen token");
     const int T = int(n);
     q::Buffers& b = c->b;
-    if (c->amap_rows != T) {
-        const float* base[6] = {b.x_hi, b.x_lo, b.att_hi, b.att_lo, b.gu_hi, b.gu_lo};
-        const int cols[6] = {q::kDim, q::kDim, q::kQDim, q::kQDim, q::kFfn, q::kFfn};
-        for (int i = 0; i < 6; ++i) qck(itts::tma_make_map(&c->amap[i], base[i], T, cols[i]), "tensor map");
-        c->amap_rows = T;
-    }
+    activation_maps(c, T);
     qck(cudaEventRecord(c->ev[0], c->stream), "event");
     qck(cudaMemcpyAsync(b.ids, ids, n * 4, cudaMemcpyHostToDevice, c->stream), "prompt upload");
     put_state(c, 0, uint32_t(n), max_out);
@@ -293,6 +319,156 @@ void ensure_graph(itts_qwen_ctx* c) {
     qck(e2, "graph capture");
     c->graph = g;
     qck(cudaGraphInstantiate(&c->exec, g, 0), "graph instantiate");
+}
+
+// ---- generate_batch: the layers of run_prompt over the packed rows of several
+// requests, with their keys and values in a paged cache.
+
+void paged(int rc) {
+    if (rc != ITTS_OK) qfail(rc, itts_paged_last_error());
+}
+
+constexpr size_t kBlockFloats = size_t(q::kBlock) * q::kKvDim;  // K (or V) of a block and layer
+
+void batch_buffers(itts_qwen_ctx* c, int32_t blocks) {
+    Batch& t = c->batch;
+    if (!t.h) {
+        t.lens = c->alloc<int32_t>(q::kBatch, "batch lengths");
+        t.fresh = c->alloc<int32_t>(q::kBatch, "batch rows");
+        t.table = c->alloc<int32_t>(size_t(q::kBatch) * q::kMaxBlocks, "block tables");
+        t.count = c->alloc<int32_t>(1, "free count");
+        t.q_start = c->alloc<int32_t>(q::kBatch + 1, "row starts");
+        t.positions = c->alloc<int32_t>(q::kStepRows, "positions");
+        t.slots = c->alloc<int32_t>(q::kStepRows, "slots");
+        t.status = c->alloc<int32_t>(1, "table status");
+        t.st = c->alloc<q::State>(q::kBatch, "batch states");
+        t.out = c->alloc<uint32_t>(size_t(q::kBatch) * q::kMaxGenerate, "batch ids");
+        t.workspace = c->alloc<unsigned char>(itts_paged_attention_workspace(q::kHeadDim), "attention workspace");
+        void* h = nullptr;
+        qck(cudaMallocHost(&h, sizeof(Batch::Host)), "pinned batch state");
+        t.h = static_cast<Batch::Host*>(h);
+    }
+    if (blocks > t.blocks) {
+        if (t.kv) cudaFree(t.kv);
+        if (t.free_list) cudaFree(t.free_list);
+        t.kv = nullptr;
+        t.free_list = nullptr;
+        t.blocks = 0;
+        t.kv = dalloc<float>(size_t(q::kLayers) * 2 * blocks * kBlockFloats, "paged KV cache");
+        t.free_list = dalloc<int32_t>(blocks, "free list");
+        t.blocks = blocks;
+    }
+    // every call starts with all blocks free
+    std::vector<int32_t> ids(t.blocks);
+    for (int32_t i = 0; i < t.blocks; ++i) ids[i] = t.blocks - 1 - i;
+    qck(cudaMemcpyAsync(t.free_list, ids.data(), ids.size() * 4, cudaMemcpyHostToDevice, c->stream), "free list");
+    qck(cudaMemcpyAsync(t.count, &t.blocks, 4, cudaMemcpyHostToDevice, c->stream), "free list");
+    qck(cudaMemsetAsync(t.lens, 0, q::kBatch * 4, c->stream), "batch lengths");
+    qck(cudaStreamSynchronize(c->stream), "free list");
+}
+
+itts_paged_cache layer_cache(const itts_qwen_ctx* c, int layer) {
+    const Batch& t = c->batch;
+    float* k = t.kv + size_t(layer) * 2 * t.blocks * kBlockFloats;
+    itts_paged_cache p{};
+    p.k = k;
+    p.v = k + size_t(t.blocks) * kBlockFloats;
+    p.type = ITTS_PAGED_F32;
+    p.blocks = t.blocks;
+    p.block_size = q::kBlock;
+    p.heads = q::kKvHeads;
+    p.head_dim = q::kHeadDim;
+    p.k_block_stride = p.v_block_stride = kBlockFloats;
+    p.k_token_stride = p.v_token_stride = q::kKvDim;
+    p.k_head_stride = p.v_head_stride = q::kHeadDim;
+    return p;
+}
+
+// One step: fresh[b] rows of request b (-1: its blocks go back), T in all, their
+// ids in h->ids.  Request b's next id is selected from its last row if pick[b].
+void run_step(itts_qwen_ctx* c, int T, const bool* pick) {
+    Batch& t = c->batch;
+    q::Buffers b = c->b;
+    cudaStream_t s = c->stream;
+    int most = 1;
+    for (int i = 0; i < q::kBatch; ++i) most = std::max(most, int(t.h->fresh[i]));
+    qck(cudaMemcpyAsync(t.fresh, t.h->fresh, q::kBatch * 4, cudaMemcpyHostToDevice, s), "batch rows");
+    itts_paged_tables_args ta{};
+    ta.requests = q::kBatch;
+    ta.block_size = q::kBlock;
+    ta.blocks = t.blocks;
+    ta.max_blocks = q::kMaxBlocks;
+    ta.table_stride = q::kMaxBlocks;
+    ta.rows = q::kStepRows;
+    ta.cached = t.lens;
+    ta.fresh = t.fresh;
+    ta.table = t.table;
+    ta.free_list = t.free_list;
+    ta.free_in = ta.free_out = t.count;
+    ta.q_start = t.q_start;
+    ta.positions = t.positions;
+    ta.slots = t.slots;
+    ta.status = t.status;
+    ta.lens = t.lens;
+    paged(itts_paged_tables(c->device, &ta, s));
+    if (T > 0) {
+        activation_maps(c, T);
+        qck(cudaMemcpyAsync(b.ids, t.h->ids, size_t(T) * 4, cudaMemcpyHostToDevice, s), "batch ids");
+        qck(cudaMemsetAsync(c->counters, 0, kCounters * 4, s), "GEMM counters");
+        qck(q::launch_embed(c->w, b, T, s), "embedding");
+        for (int l = 0; l < q::kLayers; ++l) {
+            const q::LayerW& L = c->w.layer[l];
+            const itts_paged_cache cache = layer_cache(c, l);
+            qck(q::launch_rmsnorm_split(b.hidden, L.ln1, b.x_hi, b.x_lo, T, s), "rmsnorm");
+            gemm(c, l, kMatQkv, &c->amap[0], itts::TmaEpiBias, nullptr, b.qkv, nullptr, T);
+            qck(q::launch_qk_norm_rope_rows(L, b, t.positions, T, s), "q/k norm + rope");
+            itts_paged_append_args pa{};
+            pa.cache = cache;
+            pa.k = b.qkv + q::kQDim;
+            pa.v = b.qkv + q::kQDim + q::kKvDim;
+            pa.source_type = ITTS_PAGED_F32;
+            pa.rows = T;
+            pa.k_row_stride = pa.v_row_stride = q::kQkv;
+            pa.k_head_stride = pa.v_head_stride = q::kHeadDim;
+            pa.slots = t.slots;
+            paged(itts_paged_append(c->device, &pa, s));
+            itts_paged_attention_args aa{};
+            aa.cache = cache;
+            aa.q = b.qkv;
+            aa.out = b.gu_hi;  // free until the gate|up GEMM
+            aa.q_heads = q::kQHeads;
+            aa.rows = T;
+            aa.q_row_stride = q::kQkv;
+            aa.out_row_stride = q::kQDim;
+            aa.q_head_stride = aa.out_head_stride = q::kHeadDim;
+            aa.q_start = t.q_start;
+            aa.lens = t.lens;
+            aa.table = t.table;
+            aa.table_stride = aa.max_blocks = q::kMaxBlocks;
+            aa.requests = q::kBatch;
+            aa.max_fresh = most;
+            aa.scale = 0.08838834764831844f;  // 1 / sqrt(128)
+            aa.workspace = t.workspace;
+            aa.workspace_bytes = itts_paged_attention_workspace(q::kHeadDim);
+            paged(itts_paged_attention(c->device, &aa, s));
+            qck(itts::tma_split(b.gu_hi, b.att_hi, b.att_lo, size_t(T) * q::kQDim, s), "attention split");
+            gemm(c, l, kMatO, &c->amap[2], itts::TmaEpiResid, b.hidden, b.hidden, nullptr, T);
+            qck(q::launch_rmsnorm_split(b.hidden, L.ln2, b.x_hi, b.x_lo, T, s), "rmsnorm");
+            gemm(c, l, kMatGu, &c->amap[0], itts::TmaEpiSwiGLU, nullptr, b.gu_hi, b.gu_lo, T);
+            gemm(c, l, kMatDown, &c->amap[4], itts::TmaEpiResid, b.hidden, b.hidden, nullptr, T);
+        }
+        for (int i = 0, row = 0; i < q::kBatch; ++i) {
+            row += std::max(0, int(t.h->fresh[i]));
+            if (!pick[i]) continue;
+            b.st = t.st + i;
+            b.out = t.out + size_t(i) * q::kMaxGenerate;
+            qck(q::launch_head(c->w, b, b.hidden + size_t(row - 1) * q::kDim, false, s), "head");
+        }
+    }
+    qck(cudaMemcpyAsync(t.h->st, t.st, sizeof t.h->st, cudaMemcpyDeviceToHost, s), "state read");
+    qck(cudaMemcpyAsync(&t.h->status, t.status, 4, cudaMemcpyDeviceToHost, s), "table status");
+    qck(cudaStreamSynchronize(s), "qwen step");
+    if (t.h->status) qfail(ITTS_ERR_RUNTIME, "Qwen block tables failed (status " + std::to_string(t.h->status) + ")");
 }
 
 void check_status(itts_qwen_ctx* c) {
@@ -440,6 +616,102 @@ int itts_qwen_generate(itts_qwen_ctx* ctx, const uint32_t* ids, size_t n, uint32
         *n_out = st.n_out;
         if (sel.empty() || sel.back() != q::kEos)
             qfail(ITTS_ERR_RUNTIME, "Qwen did not reach EOS within 1024 generated tokens");
+    });
+}
+
+int itts_qwen_generate_batch(itts_qwen_ctx* ctx, size_t n, const uint32_t* const* ids, const size_t* n_ids,
+                             uint32_t maximum, uint32_t* out, uint32_t* n_out, int32_t* stopped) {
+    if (!ctx) return ITTS_ERR_INVALID_ARGUMENT;
+    return qguard(ctx, [&] {
+        qck(cudaSetDevice(ctx->device), "cudaSetDevice");
+        if (n == 0) return;
+        if (!ids || !n_ids || !out || !n_out || !stopped) invalid("null argument");
+        std::vector<int32_t> need(n);  // blocks that request i may come to hold
+        uint32_t prompt = 0;
+        for (size_t i = 0; i < n; ++i) {
+            if (!maximum || maximum > uint32_t(q::kMaxGenerate) || n_ids[i] > size_t(q::kCap) ||
+                n_ids[i] + maximum > size_t(q::kCap))
+                invalid("Qwen generation capacity exceeded");
+            if (!ids[i] || n_ids[i] == 0 || n_ids[i] > size_t(q::kMaxPrompt)) invalid("Qwen prompt capacity is 3072 tokens");
+            for (size_t j = 0; j < n_ids[i]; ++j)
+                if (ids[i][j] >= uint32_t(q::kVocab)) invalid("Invalid Qwen token");
+            need[i] = int32_t((n_ids[i] + maximum + q::kBlock - 1) / q::kBlock);
+            prompt += uint32_t(n_ids[i]);
+        }
+        std::vector<int32_t> largest(need);
+        std::sort(largest.begin(), largest.end(), [](int32_t a, int32_t b) { return a > b; });
+        int32_t blocks = 0;  // whichever requests are in flight together fit
+        for (size_t i = 0; i < std::min<size_t>(n, q::kBatch); ++i) blocks += largest[i];
+        batch_buffers(ctx, blocks);
+
+        struct Place {
+            size_t request = 0, fed = 0;
+            uint32_t next = 0;  // id to feed once the prompt is
+            enum { kFree, kRunning, kRelease } state = kFree;
+        } place[q::kBatch];
+        Batch::Host& h = *ctx->batch.h;
+        size_t started = 0, finished = 0;
+        uint32_t steps = 0;
+        qck(cudaEventRecord(ctx->ev[0], ctx->stream), "event");
+        while (finished < n) {
+            int left = q::kStepRows, T = 0;
+            bool pick[q::kBatch] = {};
+            for (int i = 0; i < q::kBatch; ++i) {
+                Place& p = place[i];
+                if (p.state == Place::kFree && started < n) {
+                    p = Place{started++, 0, 0, Place::kRunning};
+                    h.st[i] = q::State{0, 0, 0, 0, maximum, {0, 0, 0}};
+                    qck(cudaMemcpyAsync(ctx->batch.st + i, &h.st[i], sizeof(q::State), cudaMemcpyHostToDevice, ctx->stream),
+                        "state upload");
+                }
+                if (p.state == Place::kRunning && p.fed >= n_ids[p.request]) --left;  // a row for each that generates
+            }
+            for (int i = 0; i < q::kBatch; ++i) {
+                Place& p = place[i];
+                h.fresh[i] = 0;
+                if (p.state == Place::kRelease) {
+                    h.fresh[i] = -1;
+                    p.state = Place::kFree;
+                    continue;
+                }
+                if (p.state != Place::kRunning) continue;
+                const size_t len = n_ids[p.request];
+                if (p.fed >= len) {
+                    h.fresh[i] = 1;
+                    h.ids[T++] = p.next;
+                    ++p.fed;
+                    pick[i] = true;
+                } else {
+                    const int rows = int(std::min<size_t>(len - p.fed, size_t(left)));
+                    std::memcpy(h.ids + T, ids[p.request] + p.fed, size_t(rows) * 4);
+                    h.fresh[i] = rows;
+                    T += rows;
+                    left -= rows;
+                    p.fed += size_t(rows);
+                    pick[i] = rows > 0 && p.fed == len;
+                }
+            }
+            run_step(ctx, T, pick);
+            if (T > 0) ++steps;
+            for (int i = 0; i < q::kBatch; ++i) {
+                if (!pick[i]) continue;
+                Place& p = place[i];
+                const q::State& st = h.st[i];
+                p.next = st.token;
+                if (!st.done) continue;
+                qck(cudaMemcpy(out + p.request * maximum, ctx->batch.out + size_t(i) * q::kMaxGenerate,
+                               size_t(st.n_out) * 4, cudaMemcpyDeviceToHost),
+                    "ids read");
+                n_out[p.request] = st.n_out;
+                stopped[p.request] = st.token == q::kEos;
+                p.state = Place::kRelease;
+                ++finished;
+            }
+        }
+        qck(cudaEventRecord(ctx->ev[1], ctx->stream), "event");
+        qck(cudaEventSynchronize(ctx->ev[1]), "qwen");
+        check_status(ctx);
+        ctx->timing = itts_qwen_timing{0.f, elapsed(ctx->ev[0], ctx->ev[1]), steps, prompt};
     });
 }
 

@@ -84,10 +84,13 @@ __global__ void __launch_bounds__(256) k_rmsnorm_split(const float* __restrict__
 // Per-head RMSNorm (q_norm / k_norm, width 128) and RoPE of token t's 16
 // query heads (in place) and 8 key heads (into the K cache at position
 // pos0 + t, with the token's value row into the V cache).  CTA = (t, head):
-// heads 0-15 query, 16-23 key.
+// heads 0-15 query, 16-23 key.  With `positions` (rows of several requests)
+// row t stands at positions[t] and its keys are rotated in place too: the
+// paged append takes them from there.
 __global__ void __launch_bounds__(128) k_qk_norm_rope(float* __restrict__ qkv, const float* __restrict__ qn,
                                                       const float* __restrict__ kn, float* __restrict__ kc,
-                                                      float* __restrict__ vc, int pos0, const State* st) {
+                                                      float* __restrict__ vc, int pos0,
+                                                      const int* __restrict__ positions, const State* st) {
     __shared__ float xs[kHeadDim];
     __shared__ float red[4];
     if (st) {
@@ -104,10 +107,10 @@ __global__ void __launch_bounds__(128) k_qk_norm_rope(float* __restrict__ qkv, c
     const float xn = x * inv * (isq ? qn : kn)[d];
     xs[d] = xn;
     __syncthreads();
-    const float angle = float(pos0 + t) * c_inv_freq[d & 63];
+    const float angle = float(positions ? positions[t] : pos0 + t) * c_inv_freq[d & 63];
     const float rot = d < 64 ? -xs[d + 64] : xs[d - 64];
     const float r = xn * cosf(angle) + rot * sinf(angle);
-    if (isq) {
+    if (isq || positions) {
         vec[d] = r;
     } else {
         const size_t o = (size_t)(pos0 + t) * kKvDim + j * kHeadDim + d;
@@ -610,7 +613,14 @@ cudaError_t launch_rmsnorm_split(const float* x, const float* g, float* hi, floa
 
 cudaError_t launch_qk_norm_rope(const LayerW& L, const Buffers& b, int layer, int T, bool decode, cudaStream_t s) {
     k_qk_norm_rope<<<dim3(T, kQHeads + kKvHeads), 128, 0, s>>>(b.qkv, L.qn, L.kn, layer_k(b, layer),
-                                                                layer_v(b, layer), 0, decode ? b.st : nullptr);
+                                                                layer_v(b, layer), 0, nullptr,
+                                                                decode ? b.st : nullptr);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_qk_norm_rope_rows(const LayerW& L, const Buffers& b, const int* positions, int T, cudaStream_t s) {
+    k_qk_norm_rope<<<dim3(T, kQHeads + kKvHeads), 128, 0, s>>>(b.qkv, L.qn, L.kn, nullptr, nullptr, 0, positions,
+                                                                nullptr);
     return cudaGetLastError();
 }
 

@@ -31,6 +31,11 @@ constexpr int kMaxChunks = kCap / kAttnChunk;
 constexpr int kPartStride = 2 + kHeadDim;  // max, sum, 128 outputs
 constexpr int kGemvRows = 8;     // rows per CTA of the decode GEMVs (one per warp)
 constexpr int kHeadCtas = kVocab / kGemvRows;
+// generate_batch: requests in flight, rows of a step, tokens of a cache block and blocks of the longest request.
+constexpr int kBatch = 16;
+constexpr int kStepRows = 1024;
+constexpr int kBlock = 64;
+constexpr int kMaxBlocks = kCap / kBlock;
 
 struct LayerW {
     const float *ln1, *ln2, *qn, *kn;
@@ -78,6 +83,8 @@ cudaError_t prepare_kernels();  // shared-memory attributes of the attention ker
 cudaError_t launch_embed(const Weights& w, const Buffers& b, int T, cudaStream_t s);
 cudaError_t launch_rmsnorm_split(const float* x, const float* g, float* hi, float* lo, int T, cudaStream_t s);
 cudaError_t launch_qk_norm_rope(const LayerW& L, const Buffers& b, int layer, int T, bool decode, cudaStream_t s);
+// The same for rows of several requests at positions[0 .. T), keys left in b.qkv.
+cudaError_t launch_qk_norm_rope_rows(const LayerW& L, const Buffers& b, const int* positions, int T, cudaStream_t s);
 cudaError_t launch_attn_prefill(const Buffers& b, int layer, int T, cudaStream_t s);
 cudaError_t launch_decode_layer(const LayerW& L, const Buffers& b, int layer, cudaStream_t s);
 cudaError_t launch_head(const Weights& w, const Buffers& b, const float* last_row, bool decode, cudaStream_t s);

@@ -109,6 +109,7 @@ SIGNATURES = {
     "itts_qwen_prefill": (C.c_int, [_P, _P, C.c_size_t, _P]),
     "itts_qwen_step": (C.c_int, [_P, C.c_uint32, _P]),
     "itts_qwen_generate": (C.c_int, [_P, _P, C.c_size_t, C.c_uint32, _P, C.c_size_t, C.POINTER(C.c_uint32)]),
+    "itts_qwen_generate_batch": (C.c_int, [_P, C.c_size_t, _P, _P, C.c_uint32, _P, _P, _P]),
     "itts_qwen_cached_tokens": (C.c_uint32, [_P]),
     "itts_qwen_last_timing": (C.c_int, [_P, _P]),
     "itts_codec_last_timing": (C.c_int, [_P, _P]),
@@ -498,6 +499,20 @@ class QwenDecoder:
         self._check(self._lib.itts_qwen_generate(self._h, _ptr(i), i.size, int(maximum), _ptr(out), out.size,
                                                  C.byref(n)))
         return out[:n.value].copy()
+
+    def generate_batch(self, prompts, maximum: int = 1024) -> list:
+        """generate() for independent prompts at once, up to 16 in flight over
+        one paged cache (itts_qwen_generate_batch): one GenerationResult per
+        prompt, ``stopped`` where its last id is EOS."""
+        ps = [_u32(p) for p in prompts]
+        b = len(ps)
+        ptrs = (C.c_void_p * max(1, b))(*[p.ctypes.data for p in ps])
+        sizes = (C.c_size_t * max(1, b))(*[p.size for p in ps])
+        out = np.zeros((max(1, b), max(1, maximum)), np.uint32)
+        n, st = np.zeros(max(1, b), np.uint32), np.zeros(max(1, b), np.int32)
+        self._check(self._lib.itts_qwen_generate_batch(self._h, b, C.cast(ptrs, C.c_void_p), C.cast(sizes, C.c_void_p),
+                                                       int(maximum), _ptr(out), _ptr(n), _ptr(st)))
+        return [GenerationResult(out[i, :n[i]].copy(), bool(st[i])) for i in range(b)]
 
     def cached_tokens(self) -> int:
         return int(self._lib.itts_qwen_cached_tokens(self._h))

@@ -152,6 +152,10 @@ def test_null_args_and_sizes(lib, gpt_mod, paged):
     assert paged.workspace_bytes(64) > 0 and paged.workspace_bytes(128) >= paged.workspace_bytes(64)
 
 
+def test_qwen_batch_needs_a_context(lib, gpt_mod):
+    assert lib.itts_qwen_generate_batch(None, 0, None, None, 8, None, None, None) == gpt_mod.ERR_INVALID_ARGUMENT
+
+
 def test_no_rows_is_no_work(lib, gpt_mod, paged):
     a = append(paged)
     a.rows = 0
