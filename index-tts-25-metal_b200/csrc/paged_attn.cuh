@@ -10,7 +10,9 @@
 // keys; an item without keys has one unit, which writes its zeros.  The lengths
 // are on the device, so the sharing-out is too: every CTA adds up the units of
 // all requests and takes an equal share [i U / n, (i + 1) U / n) of them, which
-// keeps all SMs busy whether there are many short requests or one long one.
+// keeps all SMs busy whether there are many short requests or one long one.  What
+// an item costs besides its units (its queries, its output) counts as kItem units
+// before its first one, which are shared out like the others but not worked on.
 // An item that ends up with several CTAs leaves partial sums in the workspace,
 // two slots a CTA (slot 0: the item its share begins inside of; slot 1: the
 // item that begins in it and goes on in the next); k_join adds them up in CTA
@@ -90,10 +92,10 @@ struct Request {
         return max(1, (keys<RT>(a, t) + KU - 1) / KU);
     }
     // Units of one key / value head over all tiles.
-    template <int RT, int KU>
+    template <int RT, int KU, int kItem>
     __device__ __forceinline__ long long total(const Attn& a) const {
         long long n = 0;
-        for (int t = 0; t * RT < rows; ++t) n += units<RT, KU>(a, t);
+        for (int t = 0; t * RT < rows; ++t) n += kItem + units<RT, KU>(a, t);
         return n;
     }
 };
@@ -116,7 +118,7 @@ struct PlanSmem {
 // Called by all threads of the CTA.  Returns the units of its share (0: none),
 // which is then in sm.share.  `scratch`: an int per request in shared memory,
 // used where there are more requests than threads.
-template <int RT, int KU, int kThreadsT>
+template <int RT, int KU, int kItem, int kThreadsT>
 __device__ int plan(const Attn& a, int cta, int ctas, PlanSmem<kThreadsT>& sm, int* scratch) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per = (a.requests + kThreadsT - 1) / kThreadsT, b0 = tid * per, b1 = min(a.requests, b0 + per);
@@ -125,14 +127,14 @@ __device__ int plan(const Attn& a, int cta, int ctas, PlanSmem<kThreadsT>& sm, i
     if (per == 1) {
         if (b0 < b1) {
             r.load(a, b0);
-            mine = r.total<RT, KU>(a);
+            mine = r.total<RT, KU, kItem>(a);
         }
     } else {  // coalesced loads, several in flight; then each thread adds up its requests in a row
 #pragma unroll 4
         for (int b = tid; b < a.requests; b += kThreadsT) {
             Request x;
             x.load(a, b);
-            scratch[b] = int(x.total<RT, KU>(a));
+            scratch[b] = int(x.total<RT, KU, kItem>(a));
         }
         __syncthreads();
         for (int b = b0; b < b1; ++b) mine += scratch[b];
@@ -171,27 +173,48 @@ __device__ int plan(const Attn& a, int cta, int ctas, PlanSmem<kThreadsT>& sm, i
     return int(s.u1 - s.u0);
 }
 
+// The CTA whose share holds unit u.
+__device__ __forceinline__ int cta_of(const Share& s, long long u) {
+    int i = int(u * s.ctas / s.units);
+    while (i > 0 && s.units * i / s.ctas > u) --i;
+    while (i + 1 < s.ctas && s.units * (i + 1) / s.ctas <= u) ++i;
+    return i;
+}
+
 // Walks the items of a share, unit by unit.
-template <int RT, int KU>
+template <int RT, int KU, int kItem>
 struct Walk {
     Request r;
-    int b, t, h;      // item: request, tile, kv head
-    int k, nk;        // unit of the item, units of the item
+    int b, t, h;  // item: request, tile, kv head
+    int k, nk;    // unit of the item, units of the item, the kItem first ones among them
+    int left;     // units of the share from this one on
     __device__ __forceinline__ void start(const Attn& a, const Share& s) {
         b = s.b;
         r = s.r;
         t = 0;
-        long long left = s.u0 - s.base;
+        left = int(s.u1 - s.u0);
+        long long before = s.u0 - s.base;
         for (;; ++t) {
-            nk = r.units<RT, KU>(a, t);
-            if (left < (long long)nk * a.c.heads) break;
-            left -= (long long)nk * a.c.heads;
+            nk = kItem + r.units<RT, KU>(a, t);
+            if (before < (long long)nk * a.c.heads) break;
+            before -= (long long)nk * a.c.heads;
         }
-        h = int(left / nk);
-        k = int(left - (long long)h * nk);
+        h = int(before / nk);
+        k = int(before - (long long)h * nk);
     }
-    // To the first unit of the next item (there is one).
-    __device__ __forceinline__ void next(const Attn& a) {
+    // To a unit that is worked on, this one if it is; false: the share has none left.
+    __device__ __forceinline__ bool work() {
+        if (kItem && k < kItem) {
+            left -= kItem - k;
+            k = kItem;
+        }
+        return left > 0;
+    }
+    // n units on, within the item; behind its last one to the next item.
+    __device__ __forceinline__ void advance(const Attn& a, int n) {
+        k += n;
+        left -= n;
+        if (k < nk || left <= 0) return;
         k = 0;
         if (++h < a.c.heads) return;
         h = 0;
@@ -201,17 +224,16 @@ struct Walk {
             do r.load(a, ++b);
             while (r.rows == 0);
         }
-        nk = r.units<RT, KU>(a, t);
+        nk = kItem + r.units<RT, KU>(a, t);
+    }
+    // At a unit that is worked on: the units of the item from here on in this share, and in how many shares
+    // the item is worked on if it begins here (0: all in this one; 1: it began in another).
+    __device__ __forceinline__ int run() const { return min(nk - k, left); }
+    __device__ __forceinline__ int parts(const Share& s) const {
+        if (k > kItem) return 1;
+        return run() == nk - k ? 0 : cta_of(s, s.u1 - left + (nk - k) - 1) - int(blockIdx.x) + 1;
     }
 };
-
-// The CTA whose share holds unit u.
-__device__ __forceinline__ int cta_of(const Share& s, long long u) {
-    int i = int(u * s.ctas / s.units);
-    while (i > 0 && s.units * i / s.ctas > u) --i;
-    while (i + 1 < s.ctas && s.units * (i + 1) / s.ctas <= u) ++i;
-    return i;
-}
 
 // Partial sums of an item: RT rows of D unnormalised outputs, then RT pairs
 // (maximum in units of log2, sum); slots are multiples of 128 bytes, so that the

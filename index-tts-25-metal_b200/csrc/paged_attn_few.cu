@@ -515,13 +515,13 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_attn_few(const __grid_consta
 
     pdl_trigger();
     pdl_wait();
-    const int units = plan<R, F::kUnit, kFewThreads>(a, blockIdx.x, gridDim.x, plan_smem, reinterpret_cast<int*>(ring));
+    const int units = plan<R, F::kUnit, 0, kFewThreads>(a, blockIdx.x, gridDim.x, plan_smem, reinterpret_cast<int*>(ring));
     const Share& sh = plan_smem.share;
     if (threadIdx.x == 0) put_record(a, blockIdx.x, 0, 0, 0, 0, 0);
     const int n = units;
     if (n == 0) return;
 
-    Walk<R, F::kUnit> in, at;  // of the loads and of the arithmetic
+    Walk<R, F::kUnit, 0> in, at;  // of the loads and of the arithmetic
     at.start(a, sh);
     in = at;
     int in_keys = in.r.template keys<R>(a, in.t), ids_b = -1, ids_k = 0, ids = 0;
@@ -558,8 +558,8 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_attn_few(const __grid_consta
                 cp16(dst + F::kHalf + row * (F::kChunks * 16) + (Math::kSwizzled ? swz_v<T>(row, ch) : ch) * 16,
                      v + r * a.c.v_token_stride + ch * (16 / sizeof(T)), bytes);
             }
-            if (++in.k == in.nk && i + 1 < n) {
-                in.next(a);
+            in.advance(a, 1);
+            if (in.k == 0) {
                 in_keys = in.r.template keys<R>(a, in.t);
             }
         }
@@ -596,7 +596,10 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_attn_few(const __grid_consta
 
         math.unit(my_ring + s * (2 * F::kHalf), ring_u + s * (2 * F::kHalf), key0, named, a.scale2, lane);
 
-        if (++at.k < at.nk && i + 1 < n) continue;
+        if (at.k + 1 < at.nk && i + 1 < n) {
+            at.advance(a, 1);
+            continue;
+        }
 
         // The item's keys end here, or this share does: the warps' sums meet.
         // Each warp's output goes to the stage it has just consumed.
@@ -604,7 +607,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_attn_few(const __grid_consta
         __syncwarp();
         math.end(mine, ml[warp], rows, lane);
         __syncthreads();
-        const bool whole = begun && at.k == at.nk;
+        const bool whole = begun && at.k + 1 == at.nk;
         float* slot = whole ? nullptr : part_slot<R, D>(a, blockIdx.x, begun ? 1 : 0);
         for (int x = threadIdx.x; x < rows * (D / 4); x += kFewThreads) {
             const int r = x / (D / 4), d4 = x % (D / 4);
@@ -629,11 +632,11 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_attn_few(const __grid_consta
             }
         }
         if (!whole && begun && threadIdx.x == 0) {  // it goes on: in how many shares
-            const int last = cta_of(sh, sh.u0 + i + (at.nk - at.k));
+            const int last = cta_of(sh, sh.u0 + i + (at.nk - at.k) - 1);
             put_record(a, blockIdx.x, last - int(blockIdx.x) + 1, at.h, rows, at.r.start, first);
         }
         __syncthreads();
-        if (i + 1 < n) at.next(a);
+        at.advance(a, 1);
         fresh = true;
     }
 }

@@ -56,6 +56,7 @@ constexpr int kTileThreads = 384;  // three warpgroups: 168 registers a thread a
 constexpr int kSoftmaxRegs = 208;  // ... 208 + 208 + 88 = 3 x 168 after the split
 constexpr int kOtherRegs = 88;
 constexpr int kTileCtas = 148;
+constexpr int kTileItem = 3;  // what an item costs besides its units, in units
 constexpr float kGrow = 8.f;  // log2 of the growth of the maximum that is let pass
 
 // A part of an item in this share: units [k0, k0 + n) of the item.
@@ -165,14 +166,14 @@ __device__ __forceinline__ float2 exp2_fit(float2 x) {
 // Of every kFitOf pairs of weights kFit are computed so, the rest by the exponential unit.
 constexpr int kFit = 2, kFitOf = 4;
 
-using TileWalk = Walk<kTileRows, kUnitKeys>;
-// The segment that begins at the walk's unit, which is the share's i-th.
-__device__ __forceinline__ Segment segment(const Attn& a, const TileWalk& w, const Share& sh, int i, int n) {
+using TileWalk = Walk<kTileRows, kUnitKeys, kTileItem>;
+// The segment that begins at the walk's unit.
+__device__ __forceinline__ Segment segment(const Attn& a, const TileWalk& w, const Share& sh) {
     Segment s;
     s.first = w.t * kTileRows;
     s.rows = min(kTileRows, w.r.rows - s.first);
-    s.k0 = w.k;
-    s.n = min(w.nk - w.k, n - i);
+    s.k0 = w.k - kTileItem;
+    s.n = w.run();
     s.keys = w.r.keys<kTileRows>(a, w.t);
     s.start = w.r.start;
     s.pos = w.r.len - w.r.tokens;
@@ -183,18 +184,18 @@ __device__ __forceinline__ Segment segment(const Attn& a, const TileWalk& w, con
         const int seen = min(max(w.r.pos(a, s.first + last) + 1, 0), a.cap);
         s.tu[t] = last < 128 * t ? 0 : min(max(max(1, (seen + kUnitKeys - 1) / kUnitKeys) - s.k0, 0), s.n);
     }
-    s.parts = w.k > 0 ? 1 : s.n == w.nk ? 0 : cta_of(sh, sh.u0 + i + w.nk - 1) - int(blockIdx.x) + 1;
+    s.parts = w.parts(sh);
     return s;
 }
 
 // NaN for every row of the share: what the CTA leaves when a wait has run out.
 template <class T, int D>
-__device__ __noinline__ void poison(const Attn& a, const Share& sh, int n) {
+__device__ __noinline__ void poison(const Attn& a, const Share& sh) {
     TileWalk w;
     w.start(a, sh);
     const float nan = __int_as_float(0x7fffffff);
-    for (int i = 0; i < n;) {
-        const Segment g = segment(a, w, sh, i, n);
+    while (w.work()) {
+        const Segment g = segment(a, w, sh);
         for (int x = threadIdx.x; x < g.rows * (D / 4); x += kTileThreads) {
             const int row = x / (D / 4), d4 = x % (D / 4);
             if (g.parts == 0)
@@ -204,11 +205,7 @@ __device__ __noinline__ void poison(const Attn& a, const Share& sh, int n) {
                     make_float2(0.f, nan);
         }
         if (threadIdx.x == 0 && g.parts > 1) put_record(a, blockIdx.x, g.parts, g.kvh, g.rows, g.start, g.first);
-        i += g.n;
-        if (i < n) {
-            w.k += g.n - 1;
-            w.next(a);
-        }
+        w.advance(a, g.n);
     }
 }
 
@@ -245,11 +242,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         sm.abort = 0;
     }
     pdl_wait();
-    const int units = plan<kTileRows, kUnitKeys, kTileThreads>(a, blockIdx.x, gridDim.x, sm.plan, reinterpret_cast<int*>(sm.kv));
+    const int units = plan<kTileRows, kUnitKeys, kTileItem, kTileThreads>(a, blockIdx.x, gridDim.x, sm.plan, reinterpret_cast<int*>(sm.kv));
     const Share& sh = sm.plan.share;
     if (threadIdx.x == 0) put_record(a, blockIdx.x, 0, 0, 0, 0, 0);
-    const int n = uniform(units);
-    if (n == 0) return;
+    if (units == 0) return;
     if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sm.tmem))
                      : "memory");
@@ -274,19 +270,19 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         int issued = 0;
         bool ok = true;
         const auto table_id = [&] {  // of this lane's block in the walk's unit
-            const long long page = (long long)w.k * blocks + bl;
+            const long long page = (long long)(w.k - kTileItem) * blocks + bl;
             const bool there = mine && page < (a.cap >> a.shift) && (page << a.shift) < w.r.len;
             return there ? __ldcg(a.table + w.b * a.table_stride + page) : -1;
         };
+        bool more = w.work();
         int id = table_id();
-        for (int i = 0; i < n && ok; ++i) {
+        for (int i = 0; more && ok; ++i) {
             const bool named = (unsigned)id < (unsigned)a.c.blocks;
             const unsigned bad = __ballot_sync(0xffffffffu, mine && half == 0 && !named);
             const int block = named ? id : a.c.blocks, head = w.h;
-            if (i + 1 < n) {  // the next unit's entry is under way while this one's loads are issued
-                if (++w.k == w.nk) w.next(a);
-                id = table_id();
-            }
+            w.advance(a, 1);
+            more = w.work();
+            if (more) id = table_id();  // under way while this unit's loads are issued
             if (lane == 0) *reinterpret_cast<volatile unsigned*>(&sm.bad[i & 7]) = bad;
             for (int v = 0; v < 2; ++v) {
                 const int x = 2 * i + v, s = x % NS;
@@ -315,7 +311,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 mma_ss(tmem + 128u * t, q + o, k + o, idesc16<T>(kUnitKeys, false), d > 0);
             }
         };
-        for (int i = 0, x = 0; i < n && ok; ++x) {
+        for (int i = 0, x = 0; ok; ++x) {
             ok = uniform(mbar_wait(&sm.seg_full[x % kSegments], uint32_t(x / kSegments) & 1u, &sm.abort));
             if (!ok) break;
             const Segment& sg = sm.seg[x % kSegments];
@@ -323,6 +319,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             const int tu[2] = {uniform(sg.tu[0]), uniform(sg.tu[1])};
             __syncwarp();
             if (elect()) mbar_arrive(&sm.seg_empty[x % kSegments]);
+            if (gn == 0) break;
 #pragma unroll
             for (int t = 0; t < 2 && ok; ++t)
                 if (tu[t] > 0) {
@@ -409,16 +406,19 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         w.start(a, sh);
         bool ok = true;
         int loads = 0;  // of Q tile t so far
-        for (int i = 0, x = 0; i < n && ok; ++x) {
+        for (int x = 0; ok; ++x) {
             Segment g;
             if (t == 0) {
                 if (x >= kSegments) ok = uniform(mbar_wait(&sm.seg_empty[x % kSegments], uint32_t(x / kSegments + 1) & 1u, &sm.abort));
                 if (!ok) break;
-                g = segment(a, w, sh, i, n);
+                if (w.work())
+                    g = segment(a, w, sh);
+                else
+                    g.n = 0;  // the end
                 if (lane == 0) {
                     sm.seg[x % kSegments] = g;
                     mbar_arrive(&sm.seg_full[x % kSegments]);
-                    if (g.parts > 1) put_record(a, blockIdx.x, g.parts, g.kvh, g.rows, g.start, g.first);
+                    if (g.n > 0 && g.parts > 1) put_record(a, blockIdx.x, g.parts, g.kvh, g.rows, g.start, g.first);
                 }
             } else {
                 ok = uniform(mbar_wait(&sm.seg_full[x % kSegments], uint32_t(x / kSegments) & 1u, &sm.abort));
@@ -427,6 +427,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sm.seg_empty[x % kSegments]);
             }
+            if (g.n == 0) break;
             if (g.tu[t] > 0) {
                 if (loads > 0) ok = uniform(mbar_wait(&sm.q_free[t], uint32_t(loads - 1) & 1u, &sm.abort));
                 if (!ok) break;
@@ -461,11 +462,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     if (lane == 0) mbar_arrive(&sm.q_full[t]);
                 }
             }
-            i += g.n;
-            if (t == 0 && i < n) {
-                w.k += g.n - 1;  // to the item's last unit, and over it
-                w.next(a);
-            }
+            if (t == 0) w.advance(a, g.n);
         }
         // the last load lands before the CTA may exit
         if (loads > 0 && q_tokens > 0) mbar_wait(&sm.q_full[t], uint32_t(loads - 1) & 1u, nullptr);
@@ -478,11 +475,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const uint32_t s_col = tmem + lanes + 128u * t, o_col = tmem + lanes + 256u + 128u * t;
         uint32_t ph_s = 0, ph_o = 0;
         bool ok = true;
-        for (int i = 0, x = 0; i < n; ++x) {
+        for (int i = 0, x = 0;; ++x) {
             if (ok) ok = mbar_wait(&sm.seg_full[x % kSegments], uint32_t(x / kSegments) & 1u, &sm.abort);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             const Segment& g = sm.seg[x % kSegments];
+            if (g.n == 0) break;
             const int units = g.tu[t];
             int seen = 0;  // keys of the unit that the row sees
             if (row < g.rows) seen = min(max(g.pos + over_group(a, g.first + row) + 1, 0), a.cap) - g.k0 * kUnitKeys;
@@ -622,7 +620,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         tc_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
-    if (sm.abort) poison<T, D>(a, sm.plan.share, n);
+    if (sm.abort) poison<T, D>(a, sh);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode() {

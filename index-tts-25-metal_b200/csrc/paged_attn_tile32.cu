@@ -41,6 +41,7 @@ namespace {
 constexpr int kRows32 = 128, kUnit32 = 64;
 constexpr int kThreads32 = 640;
 constexpr int kCtas32 = 148;
+constexpr int kItem32 = 3;  // what an item costs besides its units, in units
 // registers a thread after the split: 112 + 160 + 80 + 80 + 48 = 5 x 96
 constexpr int kRegsSoftmax = 112, kRegsOut = 160, kRegsSplit = 80, kRegsIssue = 48;
 constexpr int kSegments32 = 4;
@@ -54,7 +55,7 @@ struct Segment32 {
 // Where the keys of a unit lie.
 struct Unit32 {
     int ids[kUnit32 / 16];  // block of 16 keys, -1: none that the table names
-    int keys, tok, kvh;     // keys left in the item, token of the first in its block, kv head
+    int keys, tok, kvh;     // keys left in the item, token of the first in its block, kv head (-1: no unit, the end)
 };
 constexpr int kUnits32 = 8;
 
@@ -76,18 +77,18 @@ struct alignas(1024) Smem32 {
     int abort;
 };
 
-using Walk32 = Walk<kRows32, kUnit32>;
+using Walk32 = Walk<kRows32, kUnit32, kItem32>;
 
-__device__ __forceinline__ Segment32 segment32(const Attn& a, const Walk32& w, const Share& sh, int i, int n) {
+__device__ __forceinline__ Segment32 segment32(const Attn& a, const Walk32& w, const Share& sh) {
     Segment32 s;
     s.first = w.t * kRows32;
     s.rows = min(kRows32, w.r.rows - s.first);
-    s.k0 = w.k;
-    s.n = min(w.nk - w.k, n - i);
+    s.k0 = w.k - kItem32;
+    s.n = w.run();
     s.start = w.r.start;
     s.pos = w.r.len - w.r.tokens;
     s.kvh = w.h;
-    s.parts = w.k > 0 ? 1 : s.n == w.nk ? 0 : cta_of(sh, sh.u0 + i + w.nk - 1) - int(blockIdx.x) + 1;
+    s.parts = w.parts(sh);
     return s;
 }
 
@@ -113,22 +114,21 @@ __device__ __forceinline__ void split3(float x, float y, uint32_t& h, uint32_t& 
         const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&v);
     };
+    const float2 minus = make_float2(-1.f, -1.f);
     h = pack(x, y);
-    x -= __uint_as_float(h << 16);
-    y -= __uint_as_float(h & 0xffff0000u);
-    m = pack(x, y);
-    x -= __uint_as_float(m << 16);
-    y -= __uint_as_float(m & 0xffff0000u);
-    l = pack(x, y);
+    float2 r = fma2(make_float2(__uint_as_float(h << 16), __uint_as_float(h & 0xffff0000u)), minus, make_float2(x, y));
+    m = pack(r.x, r.y);
+    r = fma2(make_float2(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u)), minus, r);
+    l = pack(r.x, r.y);
 }
 
 template <int D>
-__device__ __noinline__ void poison32(const Attn& a, const Share& sh, int n) {
+__device__ __noinline__ void poison32(const Attn& a, const Share& sh) {
     Walk32 w;
     w.start(a, sh);
     const float nan = __int_as_float(0x7fffffff);
-    for (int i = 0; i < n;) {
-        const Segment32 g = segment32(a, w, sh, i, n);
+    while (w.work()) {
+        const Segment32 g = segment32(a, w, sh);
         for (int x = threadIdx.x; x < g.rows * (D / 4); x += kThreads32) {
             const int row = x / (D / 4), d4 = x % (D / 4);
             if (g.parts == 0)
@@ -138,11 +138,7 @@ __device__ __noinline__ void poison32(const Attn& a, const Share& sh, int n) {
                     make_float2(0.f, nan);
         }
         if (threadIdx.x == 0 && g.parts > 1) put_record(a, blockIdx.x, g.parts, g.kvh, g.rows, g.start, g.first);
-        i += g.n;
-        if (i < n) {
-            w.k += g.n - 1;
-            w.next(a);
-        }
+        w.advance(a, g.n);
     }
 }
 
@@ -184,11 +180,10 @@ __global__ void __launch_bounds__(kThreads32, 1) k_attn_tile32(const __grid_cons
         sm.abort = 0;
     }
     pdl_wait();
-    const int units = plan<kRows32, kUnit32, kThreads32>(a, blockIdx.x, gridDim.x, sm.plan, reinterpret_cast<int*>(sm.k));
+    const int units = plan<kRows32, kUnit32, kItem32, kThreads32>(a, blockIdx.x, gridDim.x, sm.plan, reinterpret_cast<int*>(sm.k));
     const Share& sh = sm.plan.share;
     if (threadIdx.x == 0) put_record(a, blockIdx.x, 0, 0, 0, 0, 0);
-    const int n = uniform(units);
-    if (n == 0) return;
+    if (units == 0) return;
     if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sm.tmem))
                      : "memory");
@@ -205,10 +200,11 @@ __global__ void __launch_bounds__(kThreads32, 1) k_attn_tile32(const __grid_cons
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
         const int row = threadIdx.x;
         bool ok = true;
-        for (int i = 0, x = 0; i < n; ++x) {
+        for (int i = 0, x = 0;; ++x) {
             ok = __all_sync(0xffffffffu, mbar_wait(&sm.seg_full[x % kSegments32], uint32_t(x / kSegments32) & 1u, &sm.abort));
             if (!ok) break;
             const Segment32& g = sm.seg[x % kSegments32];
+            if (g.n == 0) break;
             int seen = -g.k0 * kUnit32;  // keys of the unit that the row sees
             const bool live = row < g.rows;
             {
@@ -219,19 +215,24 @@ __global__ void __launch_bounds__(kThreads32, 1) k_attn_tile32(const __grid_cons
                                                                   (long long)(g.start + tok) * a.q_row +
                                                                   (long long)(g.kvh * a.group + r - tok * a.group) * a.q_head);
 #pragma unroll 1
-                for (int c = 0; c < D / 32; ++c) {
-                    float4 y[8];
+                for (int c = 0; c < D / 64; ++c) {  // a lane's loads fall on its own row: many in flight
+                    float4 y[16];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) y[e] = live ? __ldg(q + 8 * c + e) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    uint32_t h[16], m[16], l[16];
+                    for (int e = 0; e < 16; ++e) y[e] = live ? __ldg(q + 16 * c + e) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        split3(y[e].x * a.sign, y[e].y * a.sign, h[2 * e], m[2 * e], l[2 * e]);
-                        split3(y[e].z * a.sign, y[e].w * a.sign, h[2 * e + 1], m[2 * e + 1], l[2 * e + 1]);
+                    for (int k = 0; k < 4; ++k) {
+                        uint32_t h[8], m[8], l[8];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float4 z = y[4 * k + e];
+                            split3(z.x * a.sign, z.y * a.sign, h[2 * e], m[2 * e], l[2 * e]);
+                            split3(z.z * a.sign, z.w * a.sign, h[2 * e + 1], m[2 * e + 1], l[2 * e + 1]);
+                        }
+                        const uint32_t col = lanes + kQ + 32u * c + 8u * k;
+                        tmem_st8(col, h);
+                        tmem_st8(col + kQWord, m);
+                        tmem_st8(col + 2 * kQWord, l);
                     }
-                    tmem_st16(lanes + kQ + 16u * c, h);
-                    tmem_st16(lanes + kQ + kQWord + 16u * c, m);
-                    tmem_st16(lanes + kQ + 2 * kQWord + 16u * c, l);
                 }
                 tc_wait_st();
                 tc_before();
@@ -310,10 +311,11 @@ __global__ void __launch_bounds__(kThreads32, 1) k_attn_tile32(const __grid_cons
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsOut));
         const int row = threadIdx.x - 128;
         bool ok = true;
-        for (int i = 0, x = 0; i < n; ++x) {
+        for (int i = 0, x = 0;; ++x) {
             ok = __all_sync(0xffffffffu, mbar_wait(&sm.seg_full[x % kSegments32], uint32_t(x / kSegments32) & 1u, &sm.abort));
             if (!ok) break;
             const Segment32& g = sm.seg[x % kSegments32];
+            if (g.n == 0) break;
             float o[D];
 #pragma unroll
             for (int c = 0; c < D; ++c) o[c] = 0.f;
@@ -369,13 +371,17 @@ __global__ void __launch_bounds__(kThreads32, 1) k_attn_tile32(const __grid_cons
         const int c = warp - 8, key = 8 * c + lane / kLanes, d4 = lane % kLanes;
         float4 kr[kLoads], vr[kLoads];
         const auto load = [&](float4 (&y)[kLoads], const Unit32& w, const void* base, long long bs, long long ts, long long hs) {
-            const int id = w.ids[c >> 1], keys = id < 0 ? 0 : w.keys - key, tok = (w.tok + key) & ((1 << a.shift) - 1);
+            const int id = w.ids[c >> 1], keys = id < 0 ? 0 : w.keys - key,  // of this lane's first on
+                       tok = (w.tok + key) & ((1 << a.shift) - 1);
             const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(base) + max(id, 0) * bs + tok * ts +
                                                               w.kvh * hs) + d4;
+            const long long step = kPer * (ts / 4);
+            if (keys >= 8) {
 #pragma unroll
-            for (int e = 0; e < kLoads; ++e) {
-                y[e] = e * kPer < keys ? __ldg(p) : make_float4(0.f, 0.f, 0.f, 0.f);
-                p += kPer * (ts / 4);
+                for (int e = 0; e < kLoads; ++e) y[e] = __ldg(p + e * step);
+            } else {
+#pragma unroll
+                for (int e = 0; e < kLoads; ++e) y[e] = e * kPer < keys ? __ldg(p + e * step) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
         };
         const auto store = [&](const float4 (&y)[kLoads], unsigned char (*tile)[Smem::kWord]) {
@@ -395,13 +401,14 @@ __global__ void __launch_bounds__(kThreads32, 1) k_attn_tile32(const __grid_cons
         };
         // the unit's K and V are in registers when its turn comes, the next unit's loads follow them
         bool ok = uniform(mbar_wait(&sm.unit_full[0], 0u, &sm.abort));
+        if (ok) ok = sm.unit[0].kvh >= 0;
         if (ok) {
             load(kr, sm.unit[0], a.c.k, a.c.k_block_stride, a.c.k_token_stride, a.c.k_head_stride);
             load(vr, sm.unit[0], a.c.v, a.c.v_block_stride, a.c.v_token_stride, a.c.v_head_stride);
         }
-        for (int i = 0; i < n && ok; ++i) {
+        bool more = true;
+        for (int i = 0; more && ok; ++i) {
             const int s = i & 1;
-            const bool more = i + 1 < n;
             const Unit32& next = sm.unit[(i + 1) % kUnits32];
             if (i >= 2) ok = uniform(mbar_wait(&sm.k_empty[s], uint32_t((i >> 1) + 1) & 1u, &sm.abort));
             if (!ok) break;
@@ -411,11 +418,10 @@ __global__ void __launch_bounds__(kThreads32, 1) k_attn_tile32(const __grid_cons
             if (lane == 0) mbar_arrive(&sm.unit_empty[i % kUnits32]);
             store(kr, sm.k[s]);
             if (lane == 0) mbar_arrive(&sm.k_full[s]);
-            if (more) {
-                ok = uniform(mbar_wait(&sm.unit_full[(i + 1) % kUnits32], uint32_t((i + 1) / kUnits32) & 1u, &sm.abort));
-                if (!ok) break;
-                load(kr, next, a.c.k, a.c.k_block_stride, a.c.k_token_stride, a.c.k_head_stride);
-            }
+            ok = uniform(mbar_wait(&sm.unit_full[(i + 1) % kUnits32], uint32_t((i + 1) / kUnits32) & 1u, &sm.abort));
+            if (!ok) break;
+            more = uniform(next.kvh) >= 0;
+            if (more) load(kr, next, a.c.k, a.c.k_block_stride, a.c.k_token_stride, a.c.k_head_stride);
             if (i >= 2) ok = uniform(mbar_wait(&sm.v_empty[s], uint32_t((i >> 1) + 1) & 1u, &sm.abort));
             if (!ok) break;
             store(vr, sm.v[s]);
@@ -439,12 +445,13 @@ __global__ void __launch_bounds__(kThreads32, 1) k_attn_tile32(const __grid_cons
                 tc_commit(&sm.s_ready[u & 1]);
                 tc_commit(&sm.k_empty[u & 1]);
             };
-            for (int i = 0, x = 0; i < n && ok; ++x) {
+            for (int i = 0, x = 0; ok; ++x) {
                 ok = uniform(mbar_wait(&sm.seg_full[x % kSegments32], uint32_t(x / kSegments32) & 1u, &sm.abort));
                 if (!ok) break;
                 const int units = uniform(sm.seg[x % kSegments32].n);
                 __syncwarp();
                 if (elect()) mbar_arrive(&sm.seg_empty[x % kSegments32]);
+                if (units == 0) break;
                 ok = uniform(mbar_wait(&sm.q_full, uint32_t(x) & 1u, &sm.abort));
                 for (int j = -2; j < units && ok; ++j) {  // P V of unit j, then Q K^T of unit j + 2
                     const int u = i + j;
@@ -487,20 +494,19 @@ __global__ void __launch_bounds__(kThreads32, 1) k_attn_tile32(const __grid_cons
             Walk32 w;
             w.start(a, sh);
             bool ok = true;
-            for (int i = 0, x = 0; i < n; ++x) {
+            for (int x = 0;; ++x) {
                 if (x >= kSegments32) ok = uniform(mbar_wait(&sm.seg_empty[x % kSegments32], uint32_t(x / kSegments32 + 1) & 1u, &sm.abort));
                 if (!ok) break;
-                const Segment32 g = segment32(a, w, sh, i, n);
+                Segment32 g;
+                g.n = 0;  // the end
+                if (w.work()) g = segment32(a, w, sh);
                 if (lane == 0) {
                     sm.seg[x % kSegments32] = g;
                     mbar_arrive(&sm.seg_full[x % kSegments32]);
-                    if (g.parts > 1) put_record(a, blockIdx.x, g.parts, g.kvh, g.rows, g.start, g.first);
+                    if (g.n > 0 && g.parts > 1) put_record(a, blockIdx.x, g.parts, g.kvh, g.rows, g.start, g.first);
                 }
-                i += g.n;
-                if (i < n) {
-                    w.k += g.n - 1;  // to the item's last unit, and over it
-                    w.next(a);
-                }
+                if (g.n == 0) break;
+                w.advance(a, g.n);
             }
         } else if (warp == 18) {
             // ---- units: lane = 16 keys
@@ -508,25 +514,25 @@ __global__ void __launch_bounds__(kThreads32, 1) k_attn_tile32(const __grid_cons
             w.start(a, sh);
             int keys = w.r.keys<kRows32>(a, w.t);
             bool ok = true;
-            for (int i = 0; i < n; ++i) {
+            for (int i = 0;; ++i) {
                 const int x = i % kUnits32;
-                const int key0 = w.k * kUnit32 + 16 * lane, page = key0 >> a.shift;
+                const bool more = w.work();
+                const int first = (w.k - kItem32) * kUnit32, key0 = first + 16 * lane;
                 int id = -1;
-                if (lane < kUnit32 / 16 && key0 < keys) id = __ldcg(a.table + w.b * a.table_stride + page);
+                if (more && lane < kUnit32 / 16 && key0 < keys) id = __ldcg(a.table + w.b * a.table_stride + (key0 >> a.shift));
                 if (i >= kUnits32) ok = uniform(mbar_wait(&sm.unit_empty[x], uint32_t(i / kUnits32 + 1) & 1u, &sm.abort));
                 if (!ok) break;
                 if (lane < kUnit32 / 16) sm.unit[x].ids[lane] = (unsigned)id < (unsigned)a.c.blocks ? id : -1;
                 if (lane == 0) {
-                    sm.unit[x].keys = keys - w.k * kUnit32;
-                    sm.unit[x].tok = (w.k * kUnit32) & ((1 << a.shift) - 1);
-                    sm.unit[x].kvh = w.h;
+                    sm.unit[x].keys = keys - first;
+                    sm.unit[x].tok = first & ((1 << a.shift) - 1);
+                    sm.unit[x].kvh = more ? w.h : -1;  // -1: the end
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sm.unit_full[x]);
-                if (i + 1 < n && ++w.k == w.nk) {
-                    w.next(a);
-                    keys = w.r.keys<kRows32>(a, w.t);
-                }
+                if (!more) break;
+                w.advance(a, 1);
+                if (w.k == 0 && w.left > 0) keys = w.r.keys<kRows32>(a, w.t);
             }
         }
     }
@@ -536,7 +542,7 @@ __global__ void __launch_bounds__(kThreads32, 1) k_attn_tile32(const __grid_cons
         tc_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
-    if (sm.abort) poison32<D>(a, sm.plan.share, n);
+    if (sm.abort) poison32<D>(a, sh);
 }
 
 template <int D>
