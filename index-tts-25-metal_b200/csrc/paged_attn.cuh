@@ -100,6 +100,11 @@ struct Request {
     }
 };
 
+// a b / c for b, c < 1024, in 32 bits where they do.
+__device__ __forceinline__ long long share_of(long long a, int b, int c) {
+    return a < (1 << 22) ? (long long)(unsigned(a) * unsigned(b) / unsigned(c)) : a * b / c;
+}
+
 // The units of a launch and where this CTA's share begins.
 struct Share {
     long long units, u0, u1;  // of all items; this CTA's
@@ -157,8 +162,8 @@ __device__ int plan(const Attn& a, int cta, int ctas, PlanSmem<kThreadsT>& sm, i
     Share s{};
     s.units = all;
     s.ctas = int(min((long long)ctas, all));
-    s.u0 = cta < s.ctas ? all * cta / s.ctas : all;
-    s.u1 = cta < s.ctas ? all * (cta + 1) / s.ctas : all;
+    s.u0 = cta < s.ctas ? share_of(all, cta, s.ctas) : all;
+    s.u1 = cta < s.ctas ? share_of(all, cta + 1, s.ctas) : all;
     if (before <= s.u0 && s.u0 < before + mine) {  // one thread holds the request of u0
         s.base = before;
         s.b = b0;
@@ -173,11 +178,12 @@ __device__ int plan(const Attn& a, int cta, int ctas, PlanSmem<kThreadsT>& sm, i
     return int(s.u1 - s.u0);
 }
 
-// The CTA whose share holds unit u.
+// The CTA whose share holds unit u: the guess is at most off by its rounding.
 __device__ __forceinline__ int cta_of(const Share& s, long long u) {
-    int i = int(u * s.ctas / s.units);
-    while (i > 0 && s.units * i / s.ctas > u) --i;
-    while (i + 1 < s.ctas && s.units * (i + 1) / s.ctas <= u) ++i;
+    int i = min(s.ctas - 1, int(float(u) * float(s.ctas) / float(s.units)));
+    const long long behind = (u + 1) * s.ctas;  // share i begins at or before u: units i < behind
+    while (i > 0 && s.units * i >= behind) --i;
+    while (i + 1 < s.ctas && s.units * (i + 1) < behind) ++i;
     return i;
 }
 
@@ -199,7 +205,7 @@ struct Walk {
             if (before < (long long)nk * a.c.heads) break;
             before -= (long long)nk * a.c.heads;
         }
-        h = int(before / nk);
+        h = before < (1ll << 31) ? int(unsigned(before) / unsigned(nk)) : int(before / nk);
         k = int(before - (long long)h * nk);
     }
     // To a unit that is worked on, this one if it is; false: the share has none left.

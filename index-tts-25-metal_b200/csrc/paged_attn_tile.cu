@@ -1,36 +1,41 @@
 // Paged attention of many rows per request (prompt chunks), 16-bit types, on
 // the 5th-generation tensor cores.
 //
-// S = Q K^T and O += P V are 128 x 128 (x head_dim) tcgen05 products; bound by
-// them and, as closely, by the exponentials: a 128 x 128 tile of scores takes
-// 1024 clocks of the tensor core (both products, head_dim 128) and 1024 clocks of
-// the SM's exponential units.  So the two must run at once.  A CTA works on an
-// item of 256 rows as two tiles of 128 with a softmax warpgroup each: while
-// one tile's scores go through the exponentials, the tensor core runs the other
-// tile's P V and next Q K^T.
+// S = Q K^T and O += P V are tcgen05 products; bound by them and, as closely, by
+// the exponentials: 128 rows x 128 keys take 1024 clocks of the tensor core (both
+// products, head_dim 128) and 1024 clocks of the SM's exponential units.  A CTA
+// works on an item of 256 rows as two tiles of 128 with a softmax warpgroup each.
+// P has columns of its own, so the next unit's scores are computed as soon as this
+// unit's are read, and the softmax's chain (read the scores, maximum, exponentials,
+// write P) does not wait for the products.  To find room in the 512 columns of tensor
+// memory a unit is 64 keys with head_dim 128, 128 keys with 64.  Measured per 64 keys
+// and both tiles (head_dim 128): 1900 clocks; the exponential unit works 1024 of them,
+// the tensor core 1500 (a product of 64 keys takes it as long as one of 128, since
+// Q is read again from shared memory), the chain of a tile takes the rest of the
+// way.  With P over the scores, units of 128 keys: 3850 for 128.
+// The output is rescaled only when the maximum has grown by 2^8 or more since the last
+// time: P stays below 2^8, far from the 16-bit types' limits, and the division at the
+// end takes the same maximum out again.
+// Tried and left, as none was faster: a part of the exponentials by a polynomial on
+// the FMA units; weights with the last unit's maximum beside this unit's; two threads
+// a row (four softmax warpgroups); the tiles' exponentials in turns or out of step;
+// the next scores fetched before P is written.
 //
 // 384 threads in five roles:
-//   warps 0-3, 4-7  softmax of tile 0, 1: a thread per row (no shuffles).  Loads
-//                   its 128 scores from tensor memory, keeps the running maximum
-//                   and sum, writes P in 16 bits over the scores.  The output is
-//                   rescaled only when the maximum has grown by 2^8 or more
-//                   since the last time (P then stays below 2^8, far from
-//                   the 16-bit types' limits, and the division at the end
-//                   takes the same maximum out again).  Half of the exponentials
-//                   are computed on the FMA units (exp2_fit).  Writes the
-//                   output, or the partial sums, at an item's end.
-//   warp 8          issues the products (one lane): per unit and tile P V of this
-//                   unit, then Q K^T of the next, in that order into the same
-//                   queue, so a tile's P (which lies over its S) is consumed
-//                   before S is overwritten without a wait in between.
-//   warp 9          TMA producer: K and V blocks of a 128-key unit into a ring of
-//                   160 KB, one box per block and 64 dimensions, found through
+//   warps 0-3, 4-7  softmax of tile 0, 1: a thread per row (no shuffles); writes
+//                   the output, or the partial sums, at an item's end.
+//   warps 8, 11     issue the products of tile 0, 1: the next unit's scores when this
+//                   unit's are read, P V when P is written.  (A wait that is over
+//                   and an issue cost a warp 100 clocks and more: one warp for both
+//                   tiles was the bound, 2480 clocks for a unit of 64 keys.)
+//   warp 9          TMA producer: K and V blocks of a unit into a ring of ten 16 KB
+//                   stages, one box per block and 64 dimensions, found through
 //                   the block table; a block outside the cache reads as zeros.
-//   warps 10, 11    walk the items ahead of the others: Q of tile 0, 1 as soon as
-//                   the last Q K^T on the one before is done (TMA where the
-//                   query heads of a group divide a tile, plain loads otherwise);
-//                   warp 10 also publishes the items' extents in shared memory.
-// Tensor memory (512 columns): S / P of the tiles, O of the tiles.
+//   warp 10         walks the items ahead of the others, publishes their extents in
+//                   shared memory and loads Q of the tiles as soon as the last
+//                   scores with the one before are done (TMA where the query
+//                   heads of a group divide a tile, plain loads otherwise).
+// Tensor memory: S of the tiles, P of the tiles, O of the tiles.
 //
 // P is rounded to the 16-bit type once (V's type: the products take one type);
 // the sum is taken over the unrounded values.  That rounding is of the size of
@@ -43,6 +48,7 @@
 // Every wait is bounded; a CTA that gives up waits (bounded) for its own loads
 // and products, frees its tensor memory, writes NaN to the rows of its share and
 // returns.
+#include <algorithm>
 #include <mutex>
 
 #include "paged_tc.cuh"
@@ -51,12 +57,15 @@ namespace itts {
 namespace paged {
 namespace {
 
-constexpr int kTileRows = 256, kUnitKeys = 128;
+constexpr int kTileRows = 256;
+// Keys of a unit: 2 S + 2 P + 2 O columns are 3 keys + 2 head_dim <= 512.
+template <int D>
+constexpr int kUnitOf = D == 128 ? 64 : 128;
 constexpr int kTileThreads = 384;  // three warpgroups: 168 registers a thread at launch ...
 constexpr int kSoftmaxRegs = 208;  // ... 208 + 208 + 88 = 3 x 168 after the split
 constexpr int kOtherRegs = 88;
 constexpr int kTileCtas = 148;
-constexpr int kTileItem = 3;  // what an item costs besides its units, in units
+constexpr int kTileItem = 1;  // what an item costs besides its units, in units
 constexpr float kGrow = 8.f;  // log2 of the growth of the maximum that is let pass
 
 // A part of an item in this share: units [k0, k0 + n) of the item.
@@ -71,11 +80,12 @@ constexpr int kSegments = 4;
 template <int D>
 struct alignas(1024) TileSmem {
     static constexpr int kHalves = D / 64;
-    static constexpr int kTileBytes = kUnitKeys * D * 2;  // a K or V tile
-    static constexpr int kStages = 160 * 1024 / kTileBytes;
-    unsigned char q[2][kTileBytes];
+    static constexpr int kTileBytes = kUnitOf<D> * D * 2;  // a K or V tile
+    static constexpr int kStages = 10;
+    static constexpr int kQBytes = 128 * D * 2;
+    unsigned char q[2][kQBytes];
     unsigned char kv[kStages][kTileBytes];
-    unsigned long long full[kStages], empty[kStages], q_full[2], q_free[2], s_ready[2], p_ready[2], o_done[2], done;
+    unsigned long long full[kStages], empty[kStages], q_full[2], q_free[2], s_ready[2], s_read[2], p_ready[2], o_done[2], done[2];
     unsigned long long seg_full[kSegments], seg_empty[kSegments];
     PlanSmem<kTileThreads> plan;
     Segment seg[kSegments];
@@ -137,44 +147,18 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return d;
 }
 
-// 2^x of two values on the FMA units: x = n + f with n the nearest whole number
-// (read off the low bits of x + 1.5 2^23), 2^f by a polynomial fitted to the
-// least largest relative error on [-1/2, 1/2], n added to the exponent.  Degree
-// 3 is off by 2^-13 (bf16 rounds to 2^-9), degree 4 by 2^-18 (f16: 2^-12).
-// Below -126 the result stays at 2^-126: not for masked keys.
-template <class T>
-__device__ __forceinline__ float2 exp2_fit(float2 x) {
-    const float2 magic = make_float2(12582912.f, 12582912.f), minus = make_float2(-12582912.f, -12582912.f);
-    const float2 neg = make_float2(-1.f, -1.f);
-    x = make_float2(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
-    const float2 t = add2(x, magic), f = fma2(add2(t, minus), neg, x);
-    const auto both = [](float c) { return make_float2(c, c); };
-    float2 p;
-    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-        p = fma2(both(0.0551714934f), f, both(0.242610931f));
-        p = fma2(p, f, both(0.693260968f));
-        p = fma2(p, f, both(0.999928057f));
-    } else {
-        p = fma2(both(0.00957008637f), f, both(0.0559178516f));
-        p = fma2(p, f, both(0.240247443f));
-        p = fma2(p, f, both(0.693121791f));
-        p = fma2(p, f, both(0.999999285f));
-    }
-    return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
-                       __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
-}
-// Of every kFitOf pairs of weights kFit are computed so, the rest by the exponential unit.
-constexpr int kFit = 2, kFitOf = 4;
-
-using TileWalk = Walk<kTileRows, kUnitKeys, kTileItem>;
+template <int D>
+using TileWalk = Walk<kTileRows, kUnitOf<D>, kTileItem>;
 // The segment that begins at the walk's unit.
-__device__ __forceinline__ Segment segment(const Attn& a, const TileWalk& w, const Share& sh) {
+template <int D>
+__device__ __forceinline__ Segment segment(const Attn& a, const TileWalk<D>& w, const Share& sh) {
+    constexpr int KU = kUnitOf<D>;
     Segment s;
     s.first = w.t * kTileRows;
     s.rows = min(kTileRows, w.r.rows - s.first);
     s.k0 = w.k - kTileItem;
     s.n = w.run();
-    s.keys = w.r.keys<kTileRows>(a, w.t);
+    s.keys = w.r.template keys<kTileRows>(a, w.t);
     s.start = w.r.start;
     s.pos = w.r.len - w.r.tokens;
     s.kvh = w.h;
@@ -182,7 +166,7 @@ __device__ __forceinline__ Segment segment(const Attn& a, const TileWalk& w, con
     for (int t = 0; t < 2; ++t) {
         const int last = min(s.rows, 128 * (t + 1)) - 1;
         const int seen = min(max(w.r.pos(a, s.first + last) + 1, 0), a.cap);
-        s.tu[t] = last < 128 * t ? 0 : min(max(max(1, (seen + kUnitKeys - 1) / kUnitKeys) - s.k0, 0), s.n);
+        s.tu[t] = last < 128 * t ? 0 : min(max(max(1, (seen + KU - 1) / KU) - s.k0, 0), s.n);
     }
     s.parts = w.parts(sh);
     return s;
@@ -191,11 +175,11 @@ __device__ __forceinline__ Segment segment(const Attn& a, const TileWalk& w, con
 // NaN for every row of the share: what the CTA leaves when a wait has run out.
 template <class T, int D>
 __device__ __noinline__ void poison(const Attn& a, const Share& sh) {
-    TileWalk w;
+    TileWalk<D> w;
     w.start(a, sh);
     const float nan = __int_as_float(0x7fffffff);
     while (w.work()) {
-        const Segment g = segment(a, w, sh);
+        const Segment g = segment<D>(a, w, sh);
         for (int x = threadIdx.x; x < g.rows * (D / 4); x += kTileThreads) {
             const int row = x / (D / 4), d4 = x % (D / 4);
             if (g.parts == 0)
@@ -216,63 +200,75 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     extern __shared__ unsigned char smem_raw[];
     using Smem = TileSmem<D>;
     Smem& sm = *reinterpret_cast<Smem*>(smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023));
-    constexpr int NS = Smem::kStages, kHalves = Smem::kHalves;
+    constexpr int NS = Smem::kStages, kHalves = Smem::kHalves, KU = kUnitOf<D>, NC = KU / 32;
     constexpr uint32_t kTileBytes = Smem::kTileBytes, kHalfBytes = kTileBytes / kHalves;
+    constexpr uint32_t kQHalf = Smem::kQBytes / kHalves;
+    constexpr uint32_t kP = 2 * KU, kO = 3 * KU;  // columns of tensor memory: S of tile t at KU t, P at kP + KU / 2 t, O at kO + D t
+    static_assert(kO + 2 * D <= 512, "tensor memory");
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
 
     pdl_trigger();
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sm.tmem))
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    } else if (threadIdx.x == 320) {
+        prefetch_map(&map_k);
+        prefetch_map(&map_v);
+        if (q_tokens > 0) prefetch_map(&map_q);
+    }
     if (threadIdx.x == 0) {
         for (int s = 0; s < NS; ++s) {
             mbar_init(&sm.full[s], 1);
-            mbar_init(&sm.empty[s], 1);
+            mbar_init(&sm.empty[s], 2);  // both tiles are done with the stage
         }
         for (int t = 0; t < 2; ++t) {
             mbar_init(&sm.q_full[t], 1);
             mbar_init(&sm.q_free[t], 1);
             mbar_init(&sm.s_ready[t], 1);
+            mbar_init(&sm.s_read[t], 4);
             mbar_init(&sm.p_ready[t], 4);
             mbar_init(&sm.o_done[t], 1);
         }
         for (int x = 0; x < kSegments; ++x) {
             mbar_init(&sm.seg_full[x], 1);
-            mbar_init(&sm.seg_empty[x], 10);  // softmax warps, products, Q of tile 1
+            mbar_init(&sm.seg_empty[x], 10);  // softmax warps, products of each tile
         }
-        mbar_init(&sm.done, 1);
+        mbar_init(&sm.done[0], 1);
+        mbar_init(&sm.done[1], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         sm.abort = 0;
     }
     pdl_wait();
-    const int units = plan<kTileRows, kUnitKeys, kTileItem, kTileThreads>(a, blockIdx.x, gridDim.x, sm.plan, reinterpret_cast<int*>(sm.kv));
+    const int units = plan<kTileRows, KU, kTileItem, kTileThreads>(a, blockIdx.x, gridDim.x, sm.plan, reinterpret_cast<int*>(sm.kv));
     const Share& sh = sm.plan.share;
     if (threadIdx.x == 0) put_record(a, blockIdx.x, 0, 0, 0, 0, 0);
-    if (units == 0) return;
-    if (warp == 8) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sm.tmem))
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the plan's scratch lies where TMA writes next
     tc_before();
     __syncthreads();
     tc_after();
     const uint32_t tmem = uniform(sm.tmem);
-    // columns: S / P of tile t at 128 t, O of tile t at 256 + 128 t
+    if (units == 0) {
+        if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+        return;
+    }
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == 9) {
         // ---- TMA producer: lane = (block of the unit, 64 dimensions)
-        TileWalk w;
+        TileWalk<D> w;
         w.start(a, sh);
-        const int blocks = kUnitKeys >> a.shift, bl = lane / kHalves, half = lane % kHalves;
+        const int shift = min(a.shift, KU == 64 ? 6 : 7);  // tokens of a box: a block, or the unit's part of one
+        const int blocks = KU >> shift, bl = lane / kHalves, half = lane % kHalves;
         const bool mine = bl < blocks;
-        const uint32_t dst = half * kHalfBytes + bl * (128u << a.shift);
+        const uint32_t dst = half * kHalfBytes + bl * (128u << shift);
         int issued = 0;
         bool ok = true;
         const auto table_id = [&] {  // of this lane's block in the walk's unit
-            const long long page = (long long)(w.k - kTileItem) * blocks + bl;
-            const bool there = mine && page < (a.cap >> a.shift) && (page << a.shift) < w.r.len;
-            return there ? __ldcg(a.table + w.b * a.table_stride + page) : -1;
+            const long long key = (long long)(w.k - kTileItem) * KU + (bl << shift);
+            const bool there = mine && key < a.cap && key < w.r.len;
+            return there ? __ldcg(a.table + w.b * a.table_stride + (key >> a.shift)) : -1;
         };
         bool more = w.work();
         int id = table_id();
@@ -280,6 +276,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             const bool named = (unsigned)id < (unsigned)a.c.blocks;
             const unsigned bad = __ballot_sync(0xffffffffu, mine && half == 0 && !named);
             const int block = named ? id : a.c.blocks, head = w.h;
+            const int token = ((w.k - kTileItem) * KU) & ((1 << a.shift) - 1);  // 0 but in blocks of more than a unit
             w.advance(a, 1);
             more = w.work();
             if (more) id = table_id();  // under way while this unit's loads are issued
@@ -292,153 +289,133 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 }
                 if (lane == 0) mbar_expect(&sm.full[s], kTileBytes);
                 __syncwarp();
-                if (mine) tma_block(smem_u32(sm.kv[s]) + dst, v ? &map_v : &map_k, 64 * half, head, block, &sm.full[s]);
+                if (mine) tma_block(smem_u32(sm.kv[s]) + dst, v ? &map_v : &map_k, 64 * half, token, head, block, &sm.full[s]);
                 issued = x + 1;
             }
             ok = __all_sync(0xffffffffu, ok);
         }
         // loads still in flight land before the CTA may exit
         for (int x = max(0, issued - NS); x < issued; ++x) mbar_wait(&sm.full[x % NS], uint32_t(x / NS) & 1u, nullptr);
-    } else if (warp == 8) {
-        // ---- products
-        uint32_t ph_q[2] = {0, 0}, ph_p[2] = {0, 0};
+    } else if (warp != 10) {
+        // ---- products of tile t
+        const int t = warp == 8 ? 0 : 1;
+        uint32_t ph_q = 0, ph_p = 0;
         bool ok = true;
-        const auto scores = [&](int t, int x) {  // S of tile t from the K tile that is x-th in the ring
+        const uint32_t s_col = tmem + KU * t, p_col = tmem + kP + KU / 2 * t, o_col = tmem + kO + D * t;
+        const auto scores = [&](int x) {  // S from the K tile that is x-th in the ring
             const uint32_t q = desc_low(smem_u32(sm.q[t]), 16), k = desc_low(smem_u32(sm.kv[x % NS]), 16);
 #pragma unroll
-            for (int d = 0; d < D / 16; ++d) {
-                const uint32_t o = ((d / 4) * kHalfBytes + (d % 4) * 32u) >> 4;
-                mma_ss(tmem + 128u * t, q + o, k + o, idesc16<T>(kUnitKeys, false), d > 0);
-            }
+            for (int d = 0; d < D / 16; ++d)
+                mma_ss(s_col, q + (((d / 4) * kQHalf + (d % 4) * 32u) >> 4), k + (((d / 4) * kHalfBytes + (d % 4) * 32u) >> 4),
+                       idesc16<T>(KU, false), d > 0);
+            tc_commit(&sm.s_ready[t]);
+            tc_commit(&sm.empty[x % NS]);
         };
+        const auto output = [&](int x, bool add) {  // O += P V
+            const uint32_t v = desc_low(smem_u32(sm.kv[x % NS]), kHalfBytes);
+#pragma unroll
+            for (int k = 0; k < KU / 16; ++k)
+                mma_ts(o_col, p_col + 8u * k, v + k * (2048u >> 4), idesc16<T>(D, true), add || k > 0);
+            tc_commit(&sm.o_done[t]);
+            tc_commit(&sm.empty[x % NS]);
+        };
+        const auto wait = [&](unsigned long long* bar, uint32_t parity) {
+            ok = ok && uniform(mbar_wait(bar, parity, &sm.abort));
+            return ok;
+        };
+        const auto full = [&](int x) { return wait(&sm.full[x % NS], uint32_t(x / NS) & 1u); };
         for (int i = 0, x = 0; ok; ++x) {
-            ok = uniform(mbar_wait(&sm.seg_full[x % kSegments], uint32_t(x / kSegments) & 1u, &sm.abort));
-            if (!ok) break;
+            if (!wait(&sm.seg_full[x % kSegments], uint32_t(x / kSegments) & 1u)) break;
             const Segment& sg = sm.seg[x % kSegments];
-            const int gn = uniform(sg.n), live0 = uniform(sg.keys - sg.k0 * kUnitKeys);
-            const int tu[2] = {uniform(sg.tu[0]), uniform(sg.tu[1])};
+            const int gn = uniform(sg.n), live0 = uniform(sg.keys - sg.k0 * KU), units = uniform(sg.tu[t]);
             __syncwarp();
             if (elect()) mbar_arrive(&sm.seg_empty[x % kSegments]);
-            if (gn == 0) break;
-#pragma unroll
-            for (int t = 0; t < 2 && ok; ++t)
-                if (tu[t] > 0) {
-                    ok = uniform(mbar_wait(&sm.q_full[t], ph_q[t], &sm.abort));
-                    ph_q[t] ^= 1u;
-                }
-            ok = ok && uniform(mbar_wait(&sm.full[(2 * i) % NS], uint32_t((2 * i) / NS) & 1u, &sm.abort));
-            if (!ok) break;
-            tc_after();
-            if (elect()) {
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-                    if (tu[t] > 0) {
-                        scores(t, 2 * i);
-                        tc_commit(&sm.s_ready[t]);
-                        if (tu[t] == 1) tc_commit(&sm.q_free[t]);
-                    }
-                tc_commit(&sm.empty[(2 * i) % NS]);
-            }
             __syncwarp();
-            for (int j = 0; j < gn && ok; ++j) {
+            if (gn == 0) break;
+            if (units > 0) {
+                if (!full(2 * i) || !wait(&sm.q_full[t], ph_q)) break;
+                ph_q ^= 1u;
+                tc_after();
+                if (elect()) {
+                    scores(2 * i);
+                    if (units == 1) tc_commit(&sm.q_free[t]);
+                }
+                __syncwarp();
+            }
+            for (int j = 0; j < units; ++j) {
                 const int xv = 2 * (i + j) + 1, xk = xv + 1;
-                ok = uniform(mbar_wait(&sm.full[xv % NS], uint32_t(xv / NS) & 1u, &sm.abort));
-                if (!ok) break;
-                const uint32_t v = desc_low(smem_u32(sm.kv[xv % NS]), kHalfBytes);
-                const int live = live0 - j * kUnitKeys;
-                if (live < kUnitKeys) {  // rows behind the item's last key: zeros, whatever the cache holds
-                    for (int x = max(live, 0) * 8 + lane; x < kUnitKeys * 8; x += 32)
+                if (j + 1 < units) {
+                    if (!full(xk) || !wait(&sm.s_read[t], ph_p)) break;
+                    tc_after();
+                    if (elect()) {
+                        scores(xk);
+                        if (j + 2 == units) tc_commit(&sm.q_free[t]);
+                    }
+                    __syncwarp();
+                }
+                if (!full(xv)) break;
+                const int live = live0 - j * KU;
+                if (live < KU) {  // rows behind the item's last key: zeros (from both tiles), whatever the cache holds
+                    for (int y = max(live, 0) * 8 + lane; y < KU * 8; y += 32)
 #pragma unroll
                         for (int hf = 0; hf < kHalves; ++hf)
-                            *reinterpret_cast<uint4*>(sm.kv[xv % NS] + hf * kHalfBytes + x * 16) = make_uint4(0, 0, 0, 0);
+                            *reinterpret_cast<uint4*>(sm.kv[xv % NS] + hf * kHalfBytes + y * 16) = make_uint4(0, 0, 0, 0);
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                 }
-                bool have_k = false;
-#pragma unroll
-                for (int t = 0; t < 2 && ok; ++t) {
-                    if (j < tu[t]) {
-                        ok = uniform(mbar_wait(&sm.p_ready[t], ph_p[t], &sm.abort));
-                        ph_p[t] ^= 1u;
-                        if (!ok) break;
-                        tc_after();
-                        if (elect()) {
-#pragma unroll
-                            for (int k = 0; k < kUnitKeys / 16; ++k)
-                                mma_ts(tmem + 256u + 128u * t, tmem + 128u * t + 8u * k,
-                                       v + k * (2048u >> 4), idesc16<T>(D, true), j > 0 || k > 0);
-                            if (j + 1 == tu[t]) tc_commit(&sm.o_done[t]);
-                        }
-                        __syncwarp();
-                    }
-                    if (j + 1 < tu[t]) {
-                        if (!have_k) {
-                            have_k = true;
-                            ok = uniform(mbar_wait(&sm.full[xk % NS], uint32_t(xk / NS) & 1u, &sm.abort));
-                            if (!ok) break;
-                            tc_after();
-                        }
-                        if (elect()) {
-                            scores(t, xk);
-                            tc_commit(&sm.s_ready[t]);
-                            if (j + 2 == tu[t]) tc_commit(&sm.q_free[t]);
-                        }
-                        __syncwarp();
-                    }
-                }
-                if (ok && elect()) {
-                    tc_commit(&sm.empty[xv % NS]);
-                    if (j + 1 < gn) tc_commit(&sm.empty[xk % NS]);
+                if (!wait(&sm.p_ready[t], ph_p)) break;  // after which the unit's scores are read, too
+                ph_p ^= 1u;
+                tc_after();
+                if (elect()) output(xv, j > 0);
+                __syncwarp();
+            }
+            for (int j = units; j < gn && ok; ++j) {  // units that none of the tile's rows sees
+                const int xk = 2 * (i + j);
+                if (!full(xk) || !full(xk + 1)) break;
+                if (elect()) {
+                    mbar_arrive(&sm.empty[xk % NS]);
+                    mbar_arrive(&sm.empty[(xk + 1) % NS]);
                 }
                 __syncwarp();
             }
             i += gn;
         }
         if (elect()) {
-            tc_commit(&sm.done);  // completes when every product issued above has
-            mbar_wait(&sm.done, 0u, nullptr);
+            tc_commit(&sm.done[t]);  // completes when every product issued above has
+            mbar_wait(&sm.done[t], 0u, nullptr);
         }
         __syncwarp();
     } else {
-        // ---- segments and Q: warp 10 + t for tile t
-        const int t = warp - 10;
-        TileWalk w;
+        // ---- segments and Q
+        TileWalk<D> w;
         w.start(a, sh);
         bool ok = true;
-        int loads = 0;  // of Q tile t so far
+        int loads[2] = {0, 0};  // of Q of tile t so far
         for (int x = 0; ok; ++x) {
+            if (x >= kSegments) ok = uniform(mbar_wait(&sm.seg_empty[x % kSegments], uint32_t(x / kSegments + 1) & 1u, &sm.abort));
+            if (!ok) break;
             Segment g;
-            if (t == 0) {
-                if (x >= kSegments) ok = uniform(mbar_wait(&sm.seg_empty[x % kSegments], uint32_t(x / kSegments + 1) & 1u, &sm.abort));
-                if (!ok) break;
-                if (w.work())
-                    g = segment(a, w, sh);
-                else
-                    g.n = 0;  // the end
-                if (lane == 0) {
-                    sm.seg[x % kSegments] = g;
-                    mbar_arrive(&sm.seg_full[x % kSegments]);
-                    if (g.n > 0 && g.parts > 1) put_record(a, blockIdx.x, g.parts, g.kvh, g.rows, g.start, g.first);
-                }
-            } else {
-                ok = uniform(mbar_wait(&sm.seg_full[x % kSegments], uint32_t(x / kSegments) & 1u, &sm.abort));
-                if (!ok) break;
-                g = sm.seg[x % kSegments];
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sm.seg_empty[x % kSegments]);
+            g.n = 0;  // the end
+            if (w.work()) g = segment<D>(a, w, sh);
+            if (lane == 0) {
+                sm.seg[x % kSegments] = g;
+                mbar_arrive(&sm.seg_full[x % kSegments]);
+                if (g.n > 0 && g.parts > 1) put_record(a, blockIdx.x, g.parts, g.kvh, g.rows, g.start, g.first);
             }
             if (g.n == 0) break;
-            if (g.tu[t] > 0) {
-                if (loads > 0) ok = uniform(mbar_wait(&sm.q_free[t], uint32_t(loads - 1) & 1u, &sm.abort));
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                if (g.tu[t] == 0) continue;
+                if (loads[t] > 0) ok = uniform(mbar_wait(&sm.q_free[t], uint32_t(loads[t] - 1) & 1u, &sm.abort));
                 if (!ok) break;
-                ++loads;
+                ++loads[t];
                 const int row0 = g.first + 128 * t;
                 if (q_tokens > 0) {  // a box of q_tokens tokens and the group's heads is the tile
                     if (lane == 0) {
-                        mbar_expect(&sm.q_full[t], kTileBytes);
+                        mbar_expect(&sm.q_full[t], Smem::kQBytes);
 #pragma unroll
                         for (int hf = 0; hf < kHalves; ++hf)
-                            tma_rows(smem_u32(sm.q[t]) + hf * kHalfBytes, &map_q, 64 * hf, g.kvh * a.group,
+                            tma_rows(smem_u32(sm.q[t]) + hf * kQHalf, &map_q, 64 * hf, g.kvh * a.group,
                                      g.start + over_group(a, row0), &sm.q_full[t]);
                     }
                 } else {
@@ -455,24 +432,28 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                                                                      (long long)(g.kvh * a.group + hd) * a.q_head) + ch);
                             v = make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
                         }
-                        *reinterpret_cast<uint4*>(sm.q[t] + (ch / 8) * kHalfBytes + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = v;
+                        *reinterpret_cast<uint4*>(sm.q[t] + (ch / 8) * kQHalf + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = v;
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sm.q_full[t]);
                 }
             }
-            if (t == 0) w.advance(a, g.n);
+            w.advance(a, g.n);
         }
-        // the last load lands before the CTA may exit
-        if (loads > 0 && q_tokens > 0) mbar_wait(&sm.q_full[t], uint32_t(loads - 1) & 1u, nullptr);
+        // the last loads land before the CTA may exit
+        if (q_tokens > 0) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+                if (loads[t] > 0) mbar_wait(&sm.q_full[t], uint32_t(loads[t] - 1) & 1u, nullptr);
+        }
     }
     } else {
         // ---- softmax: tile t, a thread per row
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         const int t = warp >> 2, row = threadIdx.x;
         const uint32_t lanes = uint32_t(32 * (warp & 3)) << 16;
-        const uint32_t s_col = tmem + lanes + 128u * t, o_col = tmem + lanes + 256u + 128u * t;
+        const uint32_t s_col = tmem + lanes + KU * t, p_col = tmem + lanes + kP + KU / 2 * t, o_col = tmem + lanes + kO + D * t;
         uint32_t ph_s = 0, ph_o = 0;
         bool ok = true;
         for (int i = 0, x = 0;; ++x) {
@@ -483,85 +464,99 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             if (g.n == 0) break;
             const int units = g.tu[t];
             int seen = 0;  // keys of the unit that the row sees
-            if (row < g.rows) seen = min(max(g.pos + over_group(a, g.first + row) + 1, 0), a.cap) - g.k0 * kUnitKeys;
-            else seen = -g.k0 * kUnitKeys;
+            if (row < g.rows) seen = min(max(g.pos + over_group(a, g.first + row) + 1, 0), a.cap) - g.k0 * KU;
+            else seen = -g.k0 * KU;
             float m = -INFINITY, l = 0.f;
-            for (int j = 0; j < units; ++j, seen -= kUnitKeys) {
-                if (ok) ok = mbar_wait(&sm.s_ready[t], ph_s, &sm.abort);
+            for (int j = 0; j < units; ++j, seen -= KU) {
+                ok = mbar_wait(&sm.s_ready[t], ph_s, &sm.abort);
                 ok = __all_sync(0xffffffffu, ok);
                 ph_s ^= 1u;
                 if (!ok) break;
                 tc_after();
-                uint32_t s[4][32];
+                // chunks of 32 keys that some row of the warp sees: the others' weights are 0
+                const int chunks = min(max((__reduce_max_sync(0xffffffffu, seen) + 31) >> 5, 0), NC);
+                uint32_t s[NC][32];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld32(s_col + 32u * c, s[c]);
+                for (int c = 0; c < NC; ++c)
+                    if (c < chunks) tmem_ld32(s_col + 32u * c, s[c]);
+#pragma unroll
+                for (int c = 0; c < NC; ++c) tc_wait_ld(s[c]);
+                tc_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.s_read[t]);
                 const unsigned bad = *reinterpret_cast<volatile unsigned*>(&sm.bad[(i + j) & 7]);
-                const bool masked = __any_sync(0xffffffffu, seen < kUnitKeys) || bad;
-                const auto mask = [&](int c, uint32_t (&s)[32]) {  // a bit per key of the chunk: a block is 16 keys or more
-                    const int left = seen - 32 * c;
-                    uint32_t see = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
-                    if (bad >> (((32 * c) >> a.shift) * kHalves) & 1u) see &= 0xffff0000u;
-                    if (bad >> (((32 * c + 16) >> a.shift) * kHalves) & 1u) see &= 0x0000ffffu;
+                bool any = true;  // the row sees a key of the unit
+                if (__any_sync(0xffffffffu, seen < KU) || bad) {
+                    any = false;
+                    const int box = min(a.shift, KU == 64 ? 6 : 7);
 #pragma unroll
-                    for (int x = 0; x < 32; ++x)
-                        if (!(see >> x & 1u)) s[x] = 0xff800000u;
-                };
-                tc_wait_ld(s[0]);
+                    for (int c = 0; c < NC; ++c) {  // a bit per key of the chunk: a block is 16 keys or more
+                        const int left = seen - 32 * c;
+                        uint32_t see = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
+                        if (bad >> (((32 * c) >> box) * kHalves) & 1u) see &= 0xffff0000u;
+                        if (bad >> (((32 * c + 16) >> box) * kHalves) & 1u) see &= 0x0000ffffu;
+                        any |= see != 0u;
+                        if (__all_sync(0xffffffffu, see == 0xffffffffu)) continue;
 #pragma unroll
-                for (int c = 1; c < 4; ++c) tc_wait_ld(s[c]);
-                if (masked) {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) mask(c, s[c]);
+                        for (int e = 0; e < 32; ++e)
+                            if (!(see >> e & 1u)) s[c][e] = 0xff800000u;
+                    }
                 }
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int x = 0; x < 32; x += 2)
+                for (int c = 0; c < NC; ++c)
+                    if (c < chunks) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        mx[c] = max3(mx[c], __uint_as_float(s[c][x]), __uint_as_float(s[c][x + 1]));
+                        for (int e = 0; e < 32; e += 2)
+                            mx[e / 2 & 3] = max3(mx[e / 2 & 3], __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
+                    }
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale2;
+                // P V of the unit before is done: P may be overwritten, O rescaled
+                if (j > 0) {
+                    ok = mbar_wait(&sm.o_done[t], ph_o, &sm.abort);
+                    ok = __all_sync(0xffffffffu, ok);
+                    ph_o ^= 1u;
+                    if (!ok) break;
+                    tc_after();
+                }
                 const bool grow = top > m + kGrow || (m == -INFINITY && top > m);
                 if (__any_sync(0xffffffffu, grow)) {
                     const float mn = fmaxf(m, top), f = mn == -INFINITY ? 1.f : ex2(m - mn);
                     m = mn;
                     l *= f;
-                    if (j > 0) {  // the products of the units before are done: this unit's scores came after them
+                    if (j > 0) {
 #pragma unroll
                         for (int c = 0; c < D / 16; ++c) {
                             uint32_t o[16];
                             tmem_ld16(o_col + 16u * c, o);
                             tc_wait_ld(o);
 #pragma unroll
-                            for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
                             tmem_st16(o_col + 16u * c, o);
                         }
                     }
                 }
                 const float ref = m == -INFINITY ? 0.f : -m;
-                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
                 const float2 sc = make_float2(a.scale2, a.scale2), rf = make_float2(ref, ref);
-                const auto weights = [&](auto fit) {  // P of the unit over its scores, and its sum
+                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t p[16];
+                for (int c = 0; c < NC; ++c) {
+                    uint32_t p[16];
+                    if (c < chunks) {
 #pragma unroll
-                        for (int x = 0; x < 16; ++x) {
-                            float2 y = fma2(make_float2(__uint_as_float(s[c][2 * x]), __uint_as_float(s[c][2 * x + 1])), sc, rf);
-                            if (decltype(fit)::value && x % kFitOf < kFit)
-                                y = exp2_fit<T>(y);
-                            else
-                                y = make_float2(ex2(y.x), ex2(y.y));
-                            sum[x & 1] = add2(sum[x & 1], y);
-                            p[x] = pack16<T>(y.x, y.y);
+                        for (int e = 0; e < 16; ++e) {
+                            float2 y = fma2(make_float2(__uint_as_float(s[c][2 * e]), __uint_as_float(s[c][2 * e + 1])), sc, rf);
+                            y = make_float2(ex2(y.x), ex2(y.y));
+                            sum[e & 1] = add2(sum[e & 1], y);
+                            p[e] = pack16<T>(y.x, y.y);
                         }
-                        tmem_st16(s_col + 16u * c, p);  // over scores that this warp has read
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) p[e] = 0u;
                     }
-                };
-                if (masked)
-                    weights(std::false_type());  // a masked weight has to be 0
-                else
-                    weights(std::true_type());
-                l += (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
+                    tmem_st16(p_col + 16u * c, p);
+                }
+                if (any) l += (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
                 tc_wait_st();
                 tc_before();
                 __syncwarp();
@@ -649,7 +644,7 @@ cudaError_t launch(const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorM
 
 }  // namespace
 
-cudaError_t make_block_map(CUtensorMap* map, const itts_paged_cache& c, bool v) {
+cudaError_t make_block_map(CUtensorMap* map, const itts_paged_cache& c, bool v, int tokens) {
     const auto fn = encode();
     if (!fn) return cudaErrorNotSupported;
     const int size = c.type == ITTS_PAGED_F32 ? 4 : 2;
@@ -659,7 +654,7 @@ cudaError_t make_block_map(CUtensorMap* map, const itts_paged_cache& c, bool v) 
     const cuuint64_t strides[3] = {bytes(v ? c.v_token_stride : c.k_token_stride, c.block_size),
                                    bytes(v ? c.v_head_stride : c.k_head_stride, c.heads),
                                    bytes(v ? c.v_block_stride : c.k_block_stride, c.blocks)};
-    const cuuint32_t box[4] = {cuuint32_t(128 / size), cuuint32_t(c.block_size), 1, 1}, one[4] = {1, 1, 1, 1};
+    const cuuint32_t box[4] = {cuuint32_t(128 / size), cuuint32_t(std::min(c.block_size, tokens)), 1, 1}, one[4] = {1, 1, 1, 1};
     const CUtensorMapDataType type = c.type == ITTS_PAGED_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                      : c.type == ITTS_PAGED_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                                 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
@@ -692,7 +687,8 @@ size_t tile_workspace_floats(int head_dim) {
 // cudaErrorNotSupported: the cache's strides have no tensor map.
 cudaError_t launch_tile(const Attn& a, cudaStream_t s) {
     CUtensorMap mk, mv;
-    if (make_block_map(&mk, a.c, false) != cudaSuccess || make_block_map(&mv, a.c, true) != cudaSuccess)
+    const int unit = a.c.head_dim == 128 ? kUnitOf<128> : kUnitOf<64>;
+    if (make_block_map(&mk, a.c, false, unit) != cudaSuccess || make_block_map(&mv, a.c, true, unit) != cudaSuccess)
         return cudaErrorNotSupported;
     // Q by TMA: rows are numbered token-major, so a tile is a box of 128 / group tokens by the group's heads
     CUtensorMap mq = mk;

@@ -47,6 +47,10 @@ __device__ __forceinline__ bool mbar_wait(unsigned long long* bar, uint32_t pari
     }
 }
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
+
 // The same value in every lane, and known to be: the products' operands then
 // stay in uniform registers.
 __device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
@@ -56,13 +60,13 @@ __device__ __forceinline__ bool elect() {
     return p != 0;
 }
 
-// One block's rows of one head, 128 bytes of each (x: first element).
-__device__ __forceinline__ void tma_block(uint32_t dst, const CUtensorMap* map, int x, int head, int block,
+// Rows of one block and head from token on, 128 bytes of each (x: first element).
+__device__ __forceinline__ void tma_block(uint32_t dst, const CUtensorMap* map, int x, int token, int head, int block,
                                           unsigned long long* bar) {
     asm volatile(
         "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, "
         "%5}], [%6];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(0), "r"(head), "r"(block), "r"(smem_u32(bar))
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(token), "r"(head), "r"(block), "r"(smem_u32(bar))
         : "memory");
 }
 
@@ -167,9 +171,9 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[N])
 #undef ITTS_S32
 
 // Tensor map of a paged cache tensor: [blocks][heads][block_size][head_dim]
-// at its strides, read as boxes of one block's tokens of one head x 128 bytes,
-// 128-byte swizzled.  Blocks outside the cache read as zeros.
-cudaError_t make_block_map(CUtensorMap* map, const itts_paged_cache& c, bool v);
+// at its strides, read as boxes of up to `tokens` tokens of one block and head x
+// 128 bytes, 128-byte swizzled.  Blocks outside the cache read as zeros.
+cudaError_t make_block_map(CUtensorMap* map, const itts_paged_cache& c, bool v, int tokens);
 
 }  // namespace paged
 }  // namespace itts

@@ -580,3 +580,25 @@ def test_side_stream_is_used(paged):
         out = s.run(paged)
     side.synchronize()
     s.check(out)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("fresh", [1, 40, 200])
+@pytest.mark.parametrize("what", ["k", "v"])
+def test_attention_nan_key_reaches_every_row_that_sees_it(paged, fresh, dtype, what):
+    """A NaN in one cached key or value row, at every offset within a few blocks of keys."""
+    for j in range(64, 64 + 9):
+        s = Step([(fresh, 300)], 4, 2, 64, bs=16, dtype=dtype)
+        cache = s.kc if what == "k" else s.vc
+        cache[s.table[0, j // 16].item(), j % 16, 1, 5] = float("nan")
+        out = s.run(paged)
+        assert torch.isfinite(out[:, :2].float()).all()
+        assert torch.isnan(out[:, 2:, 5 if what == "v" else slice(None)]).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("heads,kv,dim,bs", [(16, 8, 128, 64), (12, 12, 64, 128), (6, 2, 128, 128), (20, 20, 64, 16)])
+def test_attention_many_units_per_cta(paged, heads, kv, dim, bs, dtype):
+    """Enough work that every ring of the kernels goes round several times within an item and across items."""
+    s = Step([(700, 2900), (1, 4100), (513, 1), (90, 6000), (255, 3333)], heads, kv, dim, bs=bs, dtype=dtype)
+    s.check(s.run(paged))
