@@ -30,15 +30,22 @@
 namespace itts {
 namespace paged {
 
-// Allows a kernel `bytes` of dynamic shared memory, once per device.
+// Allows a kernel `bytes` of dynamic shared memory, once per device.  regs: what a
+// kernel that shares out its registers (setmaxnreg) has to have been compiled to;
+// with fewer the shares would wait for ever.
 template <auto kKernel>
-cudaError_t allow_smem(size_t bytes) {
+cudaError_t allow_smem(size_t bytes, int regs = 0) {
     static std::atomic<uint64_t> done{0};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
     if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    if (regs) {
+        cudaFuncAttributes at{};
+        if ((e = cudaFuncGetAttributes(&at, kKernel)) != cudaSuccess) return e;
+        if (at.numRegs != regs) return cudaErrorInvalidKernelImage;
+    }
     e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
     if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
     return e;

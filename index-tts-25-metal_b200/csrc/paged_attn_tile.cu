@@ -61,9 +61,11 @@ constexpr int kTileRows = 256;
 // Keys of a unit: 2 S + 2 P + 2 O columns are 3 keys + 2 head_dim <= 512.
 template <int D>
 constexpr int kUnitOf = D == 128 ? 64 : 128;
-constexpr int kTileThreads = 384;  // three warpgroups: 168 registers a thread at launch ...
-constexpr int kSoftmaxRegs = 208;  // ... 208 + 208 + 88 = 3 x 168 after the split
-constexpr int kOtherRegs = 88;
+constexpr int kTileThreads = 384;
+// Registers a thread: 168 at launch (65536 / 384, rounded down to a multiple of 8), then by role.
+constexpr int kRegsLaunch = 168, kSoftmaxRegs = 208, kOtherRegs = 88;
+static_assert(2 * kSoftmaxRegs + kOtherRegs == 3 * kRegsLaunch && kSoftmaxRegs >= kRegsLaunch && kOtherRegs <= kRegsLaunch,
+              "more would wait for ever; inc does not lower, dec does not raise");
 constexpr int kTileCtas = 148;
 constexpr int kTileItem = 1;  // what an item costs besides its units, in units
 constexpr float kGrow = 8.f;  // log2 of the growth of the maximum that is let pass
@@ -636,7 +638,7 @@ cudaError_t launch(const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorM
                    cudaStream_t s) {
     constexpr size_t smem = sizeof(TileSmem<D>) + 1024;
     static_assert(smem <= 227 * 1024, "shared memory of a CTA");
-    cudaError_t e = allow_smem<k_attn_tile<T, D>>(smem);
+    cudaError_t e = allow_smem<k_attn_tile<T, D>>(smem, kRegsLaunch);
     if (e != cudaSuccess) return e;
     if ((e = launch_pdl(k_attn_tile<T, D>, kTileCtas, kTileThreads, smem, s, mk, mv, mq, a, q_tokens)) != cudaSuccess) return e;
     return launch_pdl(k_join_rows<T, kTileRows, D>, dim3(kTileCtas, kTileRows / join_rows(D)), kJoinThreads, 0, s, a);

@@ -42,8 +42,12 @@ constexpr int kRows32 = 128, kUnit32 = 64;
 constexpr int kThreads32 = 640;
 constexpr int kCtas32 = 148;
 constexpr int kItem32 = 3;  // what an item costs besides its units, in units
-// registers a thread after the split: 112 + 160 + 80 + 80 + 48 = 5 x 96
-constexpr int kRegsSoftmax = 112, kRegsOut = 160, kRegsSplit = 80, kRegsIssue = 48;
+// Registers a thread: 96 at launch (65536 / 640, rounded down to a multiple of 8), then by role.  K and V with 80 and
+// the softmax with 112 was 8% slower.
+constexpr int kRegsLaunch = 96, kRegsSoftmax = 104, kRegsOut = 160, kRegsSplit = 88, kRegsIssue = 40;
+static_assert(kRegsSoftmax + kRegsOut + 2 * kRegsSplit + kRegsIssue == 5 * kRegsLaunch, "more would wait for ever");
+static_assert(kRegsSoftmax >= kRegsLaunch && kRegsOut >= kRegsLaunch, "setmaxnreg.inc does not lower");
+static_assert(kRegsSplit <= kRegsLaunch && kRegsIssue <= kRegsLaunch, "setmaxnreg.dec does not raise");
 constexpr int kSegments32 = 4;
 
 struct Segment32 {
@@ -70,6 +74,8 @@ struct alignas(1024) Smem32 {
     Unit32 unit[kUnits32];
     float2 ml[4][kRows32];  // of unit j at j % 4: running maximum and sum,
     float f[4][kRows32];    // and what they rescale the output by
+    float4 turn[4][32 * 8];  // per softmax warp: 32 dimensions of its 32 rows of Q, on their way from lanes along a row
+                             // to a lane per row
     Segment32 seg[kSegments32];
     unsigned bad[4][kUnit32 / 16];  // per unit (mod 4) and 16 keys: a block that the table does not name
     PlanSmem<kThreads32> plan;
@@ -208,27 +214,43 @@ __global__ void __launch_bounds__(kThreads32, 1) k_attn_tile32(const __grid_cons
             int seen = -g.k0 * kUnit32;  // keys of the unit that the row sees
             const bool live = row < g.rows;
             {
-                const int r = g.first + row, tok = over_group(a, r);
-                if (live) seen += min(max(g.pos + tok + 1, 0), a.cap);
-                // every product with the Q before is done: the last unit's scores were read
-                const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(a.q) +
-                                                                  (long long)(g.start + tok) * a.q_row +
-                                                                  (long long)(g.kvh * a.group + r - tok * a.group) * a.q_head);
+                if (live) seen += min(max(g.pos + over_group(a, g.first + row) + 1, 0), a.cap);
+                // Q, every product with the one before being done (the last unit's scores were read).  Eight lanes
+                // load 128 bytes of a row (a lane per row would fetch every sector twice: with 200 KB of it shared
+                // memory leaves no cache to speak of), and the rows turn in shared memory.
+                const int r8 = lane >> 3, c8 = lane & 7;
+                const float* base[8];  // of rows r8, r8 + 4, ..
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int rr = 32 * warp + 4 * e + r8, at = g.first + rr, tk = over_group(a, at);
+                    base[e] = rr < g.rows ? static_cast<const float*>(a.q) + (long long)(g.start + tk) * a.q_row +
+                                                (long long)(g.kvh * a.group + at - tk * a.group) * a.q_head
+                                          : nullptr;
+                }
+                float4 y[8];
+                const auto load = [&](int c) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        y[e] = base[e] ? __ldg(reinterpret_cast<const float4*>(base[e]) + 8 * c + c8) : make_float4(0.f, 0.f, 0.f, 0.f);
+                };
+                load(0);
 #pragma unroll 1
-                for (int c = 0; c < D / 64; ++c) {  // a lane's loads fall on its own row: many in flight
-                    float4 y[16];
+                for (int c = 0; c < D / 32; ++c) {
+                    __syncwarp();
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) y[e] = live ? __ldg(q + 16 * c + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int e = 0; e < 8; ++e) sm.turn[warp][(4 * e + r8) * 8 + (c8 ^ ((4 * e + r8) & 7))] = y[e];
+                    __syncwarp();
+                    if (c + 1 < D / 32) load(c + 1);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
+                    for (int k = 0; k < 2; ++k) {
                         uint32_t h[8], m[8], l[8];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const float4 z = y[4 * k + e];
+                            const float4 z = sm.turn[warp][lane * 8 + ((4 * k + e) ^ (lane & 7))];
                             split3(z.x * a.sign, z.y * a.sign, h[2 * e], m[2 * e], l[2 * e]);
                             split3(z.z * a.sign, z.w * a.sign, h[2 * e + 1], m[2 * e + 1], l[2 * e + 1]);
                         }
-                        const uint32_t col = lanes + kQ + 32u * c + 8u * k;
+                        const uint32_t col = lanes + kQ + 16u * c + 8u * k;
                         tmem_st8(col, h);
                         tmem_st8(col + kQWord, m);
                         tmem_st8(col + 2 * kQWord, l);
@@ -549,7 +571,7 @@ template <int D>
 cudaError_t launch(const Attn& a, cudaStream_t s) {
     constexpr size_t smem = sizeof(Smem32<D>) + 1024;
     static_assert(smem <= 227 * 1024, "shared memory of a CTA");
-    cudaError_t e = allow_smem<k_attn_tile32<D>>(smem);
+    cudaError_t e = allow_smem<k_attn_tile32<D>>(smem, kRegsLaunch);
     if (e != cudaSuccess) return e;
     if ((e = launch_pdl(k_attn_tile32<D>, kCtas32, kThreads32, smem, s, a)) != cudaSuccess) return e;
     return launch_pdl(k_join_rows<float, kRows32, D>, dim3(kCtas32, kRows32 / join_rows(D)), kJoinThreads, 0, s, a);
