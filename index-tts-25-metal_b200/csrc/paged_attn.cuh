@@ -295,29 +295,27 @@ __device__ __forceinline__ float4 normalised(float4 o, float l) {
     return make_float4(o.x * i, o.y * i, o.z * i, o.w * i);
 }
 
-// Adds up the partial sums of the items that several CTAs worked on: CTA i
-// takes the item that begins in share i, if it goes on in other shares.
+// Adds up the partial sums of the items that several CTAs worked on: CTA (i, r)
+// takes rows r, r + gridDim.y, .. of the item that begins in share i, if it goes on
+// in other shares.  Groups of D / 4 threads take every gth part each.
 constexpr int kJoinThreads = 256;
 template <class T, int RT, int D>
 __global__ void __launch_bounds__(kJoinThreads) k_join(Attn a) {
     pdl_wait();
     pdl_trigger();
-    const int cta = blockIdx.x;
-    const int4 rec = __ldcg(a.rec + 2 * cta);
-    if (rec.x < 2) return;
-    const int4 where = __ldcg(a.rec + 2 * cta + 1);
-    const int parts = rec.x, rows = rec.w, kvh = rec.z, start = where.x, first = where.y;
-    extern __shared__ float4 joined[];
-    // groups of D / 4 threads: each takes every gth part of a row
     constexpr int kCols = D / 4, kGroups = kJoinThreads / kCols;
-    const int col = threadIdx.x % kCols, grp = threadIdx.x / kCols;
-    __shared__ float wl[kGroups][2];
-    const auto slot = [&](int i) { return part_slot<RT, D>(a, cta + i, i == 0 ? 1 : 0); };
-    for (int row = 0; row < rows; ++row) {
+    __shared__ float4 joined[kJoinThreads];
+    __shared__ float2 ml_of[kGroups];
+    const int cta = blockIdx.x, col = threadIdx.x % kCols, grp = threadIdx.x / kCols;
+    const int4 rec = __ldcg(a.rec + 2 * cta), where = __ldcg(a.rec + 2 * cta + 1);
+    const int parts = rec.x;
+    if (parts < 2) return;
+    for (int row = blockIdx.y; row < rec.w; row += gridDim.y) {
         float m = -INFINITY, l = 0.f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
         for (int i = grp; i < parts; i += kGroups) {
-            const float* p = slot(i);
+            const float* p = part_slot<RT, D>(a, cta + i, i == 0 ? 1 : 0);
             const float2 ml = __ldcg(reinterpret_cast<const float2*>(p + RT * D) + row);
             const float4 v = __ldcg(reinterpret_cast<const float4*>(p + row * D) + col);
             const float mn = fmaxf(m, ml.x), ref = mn == -INFINITY ? 0.f : mn;
@@ -327,23 +325,22 @@ __global__ void __launch_bounds__(kJoinThreads) k_join(Attn a) {
             m = mn;
         }
         joined[threadIdx.x] = o;
-        if (col == 0) {
-            wl[grp][0] = m;
-            wl[grp][1] = l;
-        }
+        if (col == 0) ml_of[grp] = make_float2(m, l);
         __syncthreads();
         if (grp == 0) {
             float M = -INFINITY, L = 0.f;
-            for (int i = 0; i < kGroups; ++i) M = fmaxf(M, wl[i][0]);
+#pragma unroll
+            for (int i = 0; i < kGroups; ++i) M = fmaxf(M, ml_of[i].x);
             const float ref = M == -INFINITY ? 0.f : M;
             o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
             for (int i = 0; i < kGroups; ++i) {
-                const float g = ex2(wl[i][0] - ref);
+                const float g = ex2(ml_of[i].x - ref);
                 const float4 v = joined[i * kCols + col];
-                L += wl[i][1] * g;
+                L += ml_of[i].y * g;
                 o = make_float4(o.x + v.x * g, o.y + v.y * g, o.z + v.z * g, o.w + v.w * g);
             }
-            store4<T>(out_row<T>(a, start, first, row, kvh) + 4 * col, normalised(o, L));
+            store4<T>(out_row<T>(a, where.x, where.y, row, rec.z) + 4 * col, normalised(o, L));
         }
         __syncthreads();
     }

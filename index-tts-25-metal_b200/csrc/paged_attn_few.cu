@@ -33,6 +33,8 @@
 // A masked key gets p = 0; keys behind the length and keys of bad table entries
 // are not read at all (cp.async fills zeros), so nothing that lies there can
 // reach the sums.
+#include <algorithm>
+
 #include "paged_attn.cuh"
 
 namespace itts {
@@ -642,22 +644,22 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_attn_few(const __grid_consta
 }
 
 template <class T, int D, int R>
-cudaError_t launch(const Attn& a, cudaStream_t s) {
+cudaError_t launch(const Attn& a, long long rows, cudaStream_t s) {
     cudaError_t e = allow_smem<k_attn_few<T, D, R>>(kFewSmem);
     if (e != cudaSuccess) return e;
     const int ctas = 2 * 148;
     if ((e = launch_pdl(k_attn_few<T, D, R>, ctas, kFewThreads, kFewSmem, s, a)) != cudaSuccess) return e;
-    return launch_pdl(k_join<T, R, D>, ctas, kJoinThreads, kJoinThreads * sizeof(float4), s, a);
+    return launch_pdl(k_join<T, R, D>, dim3(ctas, unsigned(std::min<long long>(rows, R))), kJoinThreads, 0, s, a);
 }
 
 // The smallest R that holds `rows`; more take several tiles.
 template <int D>
 cudaError_t launch32(const Attn& a, long long rows, cudaStream_t s) {
-    if (rows <= 1) return launch<float, D, 1>(a, s);
-    if (rows <= 2) return launch<float, D, 2>(a, s);
-    if (rows <= 4) return launch<float, D, 4>(a, s);
-    if (rows <= kSimtMost) return launch<float, D, 8>(a, s);
-    return launch<float, D, kMmaRows>(a, s);
+    if (rows <= 1) return launch<float, D, 1>(a, rows, s);
+    if (rows <= 2) return launch<float, D, 2>(a, rows, s);
+    if (rows <= 4) return launch<float, D, 4>(a, rows, s);
+    if (rows <= kSimtMost) return launch<float, D, 8>(a, rows, s);
+    return launch<float, D, kMmaRows>(a, rows, s);
 }
 
 }  // namespace
@@ -671,8 +673,8 @@ cudaError_t launch_few(const Attn& a, long long rows, cudaStream_t s) {
     const bool wide = a.c.head_dim == 128;
     constexpr int R = kMmaRows;
     switch (a.c.type) {
-        case ITTS_PAGED_F16: return wide ? launch<__half, 128, R>(a, s) : launch<__half, 64, R>(a, s);
-        case ITTS_PAGED_BF16: return wide ? launch<__nv_bfloat16, 128, R>(a, s) : launch<__nv_bfloat16, 64, R>(a, s);
+        case ITTS_PAGED_F16: return wide ? launch<__half, 128, R>(a, rows, s) : launch<__half, 64, R>(a, rows, s);
+        case ITTS_PAGED_BF16: return wide ? launch<__nv_bfloat16, 128, R>(a, rows, s) : launch<__nv_bfloat16, 64, R>(a, rows, s);
         default: return wide ? launch32<128>(a, rows, s) : launch32<64>(a, rows, s);
     }
 }
