@@ -184,9 +184,19 @@ __global__ void __launch_bounds__(kTabThreads) k_tables(itts_paged_tables_args a
         a.lens[b] = !ok ? held[b] : __ldcg(a.fresh + b) < 0 ? 0 : grown;
     }
     if (ok) {
-        for (int i = me; i < int(fresh_blocks); i += step) {
-            const int b = owner([=](int b) { return new_off[b]; }, B, i), have = (held[b] + bs - 1) >> shift;
-            a.table[(long long)b * a.table_stride + have + (i - new_off[b])] = __ldcg(a.free_list + top - 1 - i);
+        constexpr int kBatch = 4;  // loads in flight: a store to the table may, for all the compiler knows, change the list
+        for (int i0 = me; i0 < int(fresh_blocks); i0 += kBatch * step) {
+            int id[kBatch];
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u)
+                if (i0 + u * step < int(fresh_blocks)) id[u] = __ldcg(a.free_list + top - 1 - (i0 + u * step));
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                const int i = i0 + u * step;
+                if (i >= int(fresh_blocks)) break;
+                const int b = owner([=](int b) { return new_off[b]; }, B, i), have = (held[b] + bs - 1) >> shift;
+                a.table[(long long)b * a.table_stride + have + (i - new_off[b])] = id[u];
+            }
         }
     }
     for (int t = me; t < map_rows; t += step) {
