@@ -71,7 +71,7 @@ typedef struct itts_paged_tables_args {
     int32_t requests;     /* 1 .. ITTS_PAGED_MAX_REQUESTS */
     int32_t block_size;   /* 16, 32, 64 or 128 */
     int32_t blocks;       /* blocks of the pool; blocks * block_size < 2^31 */
-    int32_t max_blocks;   /* columns of the table; max_blocks * block_size < 2^31 */
+    int32_t max_blocks;   /* columns of the table; max_blocks * block_size <= 2^30 */
     int64_t table_stride; /* elements between the rows of the table, >= max_blocks */
     int32_t rows;         /* entries of positions and slots, 0 .. 2^30 */
     const int32_t* cached;  /* [requests] tokens cached before the step */
@@ -135,7 +135,9 @@ int itts_paged_append(int device, const itts_paged_append_args* args, void* stre
  * table does not name, never reaches the output, NaN and infinities included.
  * A table entry outside 0 .. blocks - 1 is not followed: its keys count as not
  * seen, as do the keys behind the table's last column.  q_start values are
- * clamped to 0 .. rows.
+ * clamped to 0 .. rows.  (A NaN or infinity in a key or value makes every row
+ * that sees it NaN or infinite; in the value row of a later row of the same
+ * chunk it may reach the chunk's earlier rows, too.)
  *
  * max_fresh is a bound on the fresh rows of one request, known on the host
  * where the lengths are not.  The kernel is chosen by it; results are right
@@ -153,7 +155,7 @@ typedef struct itts_paged_attention_args {
     const int32_t* table;   /* [requests][max_blocks] */
     int64_t table_stride;
     int32_t requests;  /* 1 .. ITTS_PAGED_MAX_REQUESTS */
-    int32_t max_blocks;
+    int32_t max_blocks; /* columns of the table; max_blocks * block_size <= 2^30 */
     int32_t max_fresh; /* >= 1 */
     float scale;       /* finite */
     void* workspace;   /* 256-byte aligned; its contents before the call do not matter */

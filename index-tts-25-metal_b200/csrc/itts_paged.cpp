@@ -97,7 +97,7 @@ void check_cache(const itts_paged_cache& c) {
 void check_table(const int32_t* table, int64_t stride, int32_t requests, int32_t max_blocks, int32_t block_size) {
     check(table, "block table is null");
     check(requests >= 1 && requests <= ITTS_PAGED_MAX_REQUESTS, "requests out of range");
-    check(max_blocks >= 1 && int64_t(max_blocks) * block_size < kInt32, "block table width out of range");
+    check(max_blocks >= 1 && int64_t(max_blocks) * block_size <= kMaxRows, "block table width out of range");
     check(stride >= max_blocks && stride < kInt32, "block table stride out of range");
 }
 

@@ -16,7 +16,9 @@ size_t tile32_workspace_floats(int head_dim);
 cudaError_t launch_tile32(const Attn& a, cudaStream_t s);
 
 namespace {
-// Rows of a request and kv head up to which the streaming kernel is used.
+// Rows of a request and kv head up to which the streaming kernel is used.  Measured (us, 16 requests, streaming / tile
+// kernel), bf16, 16 heads on 8 of 128: 200 keys, 16 rows 16.0 / 18.1, 18 rows 26.5 / 18.2; 4000 keys, 16 rows 55 / 65,
+// 18 rows 96 / 65.  fp32: 16 rows 20 / 24 and 144 / 169, 18 rows 36 / 24 and 280 / 170.
 constexpr int kFewMost = 16;
 constexpr size_t kRecords = size_t(2) * kMaxCtas * sizeof(int4);
 }

@@ -25,8 +25,9 @@
 // operand's index in an order that lets a lane read four of them at once.
 //
 // Up to eight rows of 32 bits stay on the CUDA cores: there a row costs its own
-// products only, where the tile costs sixteen rows' three times over (one step of
-// 16 requests with two rows each: see kSimtMost).  A lane holds four dimensions of
+// products only, where the tile costs sixteen rows' three times over (us, 16
+// requests over 4000 keys, 16 heads on 8 of 128, CUDA cores / tile: 8 rows 98 / 139,
+// 4 rows 85 / 139).  A lane holds four dimensions of
 // every row's query and output; the partial scores of eight keys times R rows are
 // summed over the lanes by exchanging halves (one shuffle per value, not five).
 //

@@ -51,6 +51,7 @@ def refused(lib, gpt_mod, entry, args, text):
     ("blocks", 1 << 27, "cache size out of range"),
     ("max_blocks", 0, "width out of range"),
     ("max_blocks", 1 << 27, "width out of range"),
+    ("max_blocks", (1 << 26) + 1, "width out of range"),
     ("table_stride", 7, "stride out of range"),
     ("table_stride", 1 << 31, "stride out of range"),
     ("rows", -1, "rows out of range"),
