@@ -602,3 +602,56 @@ def test_attention_many_units_per_cta(paged, heads, kv, dim, bs, dtype):
     """Enough work that every ring of the kernels goes round several times within an item and across items."""
     s = Step([(700, 2900), (1, 4100), (513, 1), (90, 6000), (255, 3333)], heads, kv, dim, bs=bs, dtype=dtype)
     s.check(s.run(paged))
+
+
+# Row maps longer than one launch fills: a second grid finds each row's request.
+LONG_MAPS = {
+    "one": ([3], [16385]),
+    "few": ([3, 50, 0, 700], [9000, 1, 0, 11000]),
+    "steps": ([(11 * i) % 70 for i in range(8192)], [(i % 5) + 1 if i % 7 else 0 for i in range(8192)]),
+    "ones": ([i % 33 for i in range(8192)], [1] * 4096 + [4] * 4096),
+    "gaps": ([i % 20 for i in range(8000)],
+             [17000] + [0] * 3000 + [7] * 100 + [-1] * 3000 + [900, 0, 1] + [0] * 1800 + [5] * 96),
+}
+
+
+@pytest.mark.parametrize("pad", [0, 1, 2, 3, 1500])
+@pytest.mark.parametrize("name", LONG_MAPS)
+def test_tables_long_maps(paged, name, pad):
+    cached, fresh = LONG_MAPS[name]
+    s = TableState(cached, fresh, 64, rows=sum(max(f, 0) for f in fresh) + pad, seed=pad)
+    d = s.device()
+    run_tables(paged, d, 64)
+    s.check(d)
+
+
+@pytest.mark.parametrize("rows", [16383, 16384, 16385])
+def test_tables_long_map_edges(paged, rows):
+    s = TableState([3, 50, 0], [1, 9000, 2], 16, rows=rows)
+    d = s.device()
+    run_tables(paged, d, 16)
+    s.check(d)
+
+
+@pytest.mark.parametrize("shift", [1, 2, 3])
+@pytest.mark.parametrize("which", ["positions", "slots"])
+def test_tables_long_map_odd_addresses(paged, which, shift):
+    s = TableState([3, 50, 0], [1, 20000, 2], 16)
+    d = s.device()
+    whole = ints([99] * (s.rows + shift + 1))
+    d[which] = whole[shift:shift + s.rows]
+    run_tables(paged, d, 16)
+    s.check(d)
+    assert (whole[:shift] == 99).all() and whole[-1].item() == 99
+
+
+@pytest.mark.parametrize("name,bit,base,spoil", [f for f in failing() if f[0] in ("length", "blocks", "released")],
+                         ids=["length", "blocks", "released"])
+def test_tables_long_map_failures(paged, name, bit, base, spoil):
+    s = TableState(list(base[0]), list(base[1]), 16, columns=6, rows=20001)
+    spoil(s)
+    d = s.device()
+    run_tables(paged, d, 16)
+    assert d["status"].item() & bit
+    assert d["table"].tolist() == s.table and d["lens"].tolist() == s.cached and d["free_out"].item() == s.count
+    assert d["slots"].tolist() == [-1] * s.rows and d["positions"].tolist() == [0] * s.rows
