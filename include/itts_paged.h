@@ -139,13 +139,17 @@ int itts_paged_append(int device, const itts_paged_append_args* args, void* stre
  * that sees it NaN or infinite; in the value row of a later row of the same
  * chunk it may reach the chunk's earlier rows, too.)
  *
+ * Work beyond all measure is not begun: if the lengths ask for more than 2^29
+ * tiles (of 1 to 128 rows by 32 to 128 keys) per CTA, which is minutes, every
+ * row is left as it was.
+ *
  * max_fresh is a bound on the fresh rows of one request, known on the host
  * where the lengths are not.  The kernel is chosen by it; results are right
  * (to rounding) whatever it says. */
 typedef struct itts_paged_attention_args {
     itts_paged_cache cache;
     const void* q;   /* [rows][q_heads][head_dim] of the cache's type, head_dim contiguous */
-    void* out;       /* as q; must not overlap it unless it is q with the same strides */
+    void* out;       /* as q; must not overlap it */
     int32_t q_heads; /* a multiple of cache.heads, at most 128 times it */
     int32_t rows;    /* 0 .. 2^30, and so is rows * q_heads / heads */
     int64_t q_row_stride, q_head_stride; /* elements */

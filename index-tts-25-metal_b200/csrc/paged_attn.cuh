@@ -53,6 +53,13 @@ cudaError_t allow_smem(size_t bytes, int regs = 0) {
 
 constexpr int kMaxCtas = 592;  // of one attention launch: 148 SMs, up to four CTAs each
 constexpr float kLog2e = 1.4426950408889634f;
+// Units of one CTA beyond which a launch does nothing: minutes of work, which only lengths out of their senses ask for.
+// It keeps the counts of a share in 32 bits.
+constexpr long long kMostUnits = 1 << 29;
+// A request's units are not counted on from here: it alone is more than all CTAs take, and so is the sum over
+// 2^13 requests and 2^10 heads, which stays in 64 bits.
+constexpr long long kEnoughUnits = 1ll << 39;
+static_assert(kEnoughUnits > kMostUnits * kMaxCtas, "");
 
 // The part of the arguments that the kernels read.
 struct Attn {
@@ -102,7 +109,7 @@ struct Request {
     template <int RT, int KU, int kItem>
     __device__ __forceinline__ long long total(const Attn& a) const {
         long long n = 0;
-        for (int t = 0; t * RT < rows; ++t) n += kItem + units<RT, KU>(a, t);
+        for (int t = 0; t * RT < rows && n < kEnoughUnits; ++t) n += kItem + units<RT, KU>(a, t);
         return n;
     }
 };
@@ -128,10 +135,10 @@ struct PlanSmem {
 };
 
 // Called by all threads of the CTA.  Returns the units of its share (0: none),
-// which is then in sm.share.  `scratch`: an int per request in shared memory,
+// which is then in sm.share.  `scratch`: a count per request in shared memory,
 // used where there are more requests than threads.
 template <int RT, int KU, int kItem, int kThreadsT>
-__device__ int plan(const Attn& a, int cta, int ctas, PlanSmem<kThreadsT>& sm, int* scratch) {
+__device__ int plan(const Attn& a, int cta, int ctas, PlanSmem<kThreadsT>& sm, long long* scratch) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per = (a.requests + kThreadsT - 1) / kThreadsT, b0 = tid * per, b1 = min(a.requests, b0 + per);
     long long mine = 0;
@@ -146,7 +153,7 @@ __device__ int plan(const Attn& a, int cta, int ctas, PlanSmem<kThreadsT>& sm, i
         for (int b = tid; b < a.requests; b += kThreadsT) {
             Request x;
             x.load(a, b);
-            scratch[b] = int(x.total<RT, KU, kItem>(a));
+            scratch[b] = x.total<RT, KU, kItem>(a);
         }
         __syncthreads();
         for (int b = b0; b < b1; ++b) mine += scratch[b];
@@ -166,6 +173,7 @@ __device__ int plan(const Attn& a, int cta, int ctas, PlanSmem<kThreadsT>& sm, i
         if (w < warp) before += sm.warp_sum[w];
         all += sm.warp_sum[w];
     }
+    if (all >= kMostUnits * ctas) all = 0;
     Share s{};
     s.units = all;
     s.ctas = int(min((long long)ctas, all));
@@ -175,7 +183,7 @@ __device__ int plan(const Attn& a, int cta, int ctas, PlanSmem<kThreadsT>& sm, i
         s.base = before;
         s.b = b0;
         if (per > 1) {
-            while (s.u0 >= s.base + (long long)scratch[s.b] * a.c.heads) s.base += (long long)scratch[s.b++] * a.c.heads;
+            while (s.u0 >= s.base + scratch[s.b] * a.c.heads) s.base += scratch[s.b++] * a.c.heads;
             r.load(a, s.b);
         }
         s.r = r;

@@ -518,7 +518,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_attn_few(const __grid_consta
 
     pdl_trigger();
     pdl_wait();
-    const int units = plan<R, F::kUnit, 0, kFewThreads>(a, blockIdx.x, gridDim.x, plan_smem, reinterpret_cast<int*>(ring));
+    const int units = plan<R, F::kUnit, 0, kFewThreads>(a, blockIdx.x, gridDim.x, plan_smem, reinterpret_cast<long long*>(ring));
     const Share& sh = plan_smem.share;
     if (threadIdx.x == 0) put_record(a, blockIdx.x, 0, 0, 0, 0, 0);
     const int n = units;

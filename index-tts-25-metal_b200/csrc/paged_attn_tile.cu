@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         sm.abort = 0;
     }
     pdl_wait();
-    const int units = plan<kTileRows, KU, kTileItem, kTileThreads>(a, blockIdx.x, gridDim.x, sm.plan, reinterpret_cast<int*>(sm.kv));
+    const int units = plan<kTileRows, KU, kTileItem, kTileThreads>(a, blockIdx.x, gridDim.x, sm.plan, reinterpret_cast<long long*>(sm.kv));
     const Share& sh = sm.plan.share;
     if (threadIdx.x == 0) put_record(a, blockIdx.x, 0, 0, 0, 0, 0);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the plan's scratch lies where TMA writes next

@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(kThreads32, 1) k_attn_tile32(const __grid_cons
         sm.abort = 0;
     }
     pdl_wait();
-    const int units = plan<kRows32, kUnit32, kItem32, kThreads32>(a, blockIdx.x, gridDim.x, sm.plan, reinterpret_cast<int*>(sm.k));
+    const int units = plan<kRows32, kUnit32, kItem32, kThreads32>(a, blockIdx.x, gridDim.x, sm.plan, reinterpret_cast<long long*>(sm.k));
     const Share& sh = sm.plan.share;
     if (threadIdx.x == 0) put_record(a, blockIdx.x, 0, 0, 0, 0, 0);
     if (units == 0) return;

@@ -655,3 +655,17 @@ def test_tables_long_map_failures(paged, name, bit, base, spoil):
     assert d["status"].item() & bit
     assert d["table"].tolist() == s.table and d["lens"].tolist() == s.cached and d["free_out"].item() == s.count
     assert d["slots"].tolist() == [-1] * s.rows and d["positions"].tolist() == [0] * s.rows
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("max_fresh", [1, 32768])
+def test_attention_without_measure_is_not_begun(paged, max_fresh, dtype):
+    """Lengths of 2^30 for 32768 rows: in units of 256 rows by 64 keys, the largest, 2^7 2^24 128 = 2^38 of them, 3.5
+    times the 2^29 for each of 148 CTAs."""
+    rows, heads, dim, bs = 32768, 128, 128, 128
+    cache = torch.zeros(2, bs, heads, dim, dtype=dtype, device=DEV)
+    q = torch.zeros(1, heads, dim, dtype=dtype, device=DEV).expand(rows, heads, dim)
+    out = torch.full((rows, heads, dim), 3.0, dtype=dtype, device=DEV)
+    table = torch.full((1, 2 ** 30 // bs), -1, dtype=torch.int32, device=DEV)
+    paged.attention(q, cache, cache, table, ints([2 ** 30]), ints([0, rows]), max_fresh, out=out)
+    assert (out == 3).all()
