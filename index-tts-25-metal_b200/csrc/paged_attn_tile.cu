@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         bool ok = true;
         int loads[2] = {0, 0};  // of Q of tile t so far
         for (int x = 0; ok; ++x) {
-            if (x >= kSegments) ok = uniform(mbar_wait(&sm.seg_empty[x % kSegments], uint32_t(x / kSegments + 1) & 1u, &sm.abort));
+            if (x >= kSegments) ok = uniform(mbar_wait(&sm.seg_empty[x % kSegments], uint32_t(x / kSegments + 1) & 1u, &sm.abort, kItemLimitNs));
             if (!ok) break;
             Segment g;
             g.n = 0;  // the end
@@ -408,7 +408,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 if (g.tu[t] == 0) continue;
-                if (loads[t] > 0) ok = uniform(mbar_wait(&sm.q_free[t], uint32_t(loads[t] - 1) & 1u, &sm.abort));
+                if (loads[t] > 0) ok = uniform(mbar_wait(&sm.q_free[t], uint32_t(loads[t] - 1) & 1u, &sm.abort, kItemLimitNs));
                 if (!ok) break;
                 ++loads[t];
                 const int row0 = g.first + 128 * t;

@@ -517,7 +517,8 @@ __global__ void __launch_bounds__(kThreads32, 1) k_attn_tile32(const __grid_cons
             w.start(a, sh);
             bool ok = true;
             for (int x = 0;; ++x) {
-                if (x >= kSegments32) ok = uniform(mbar_wait(&sm.seg_empty[x % kSegments32], uint32_t(x / kSegments32 + 1) & 1u, &sm.abort));
+                if (x >= kSegments32)
+                    ok = uniform(mbar_wait(&sm.seg_empty[x % kSegments32], uint32_t(x / kSegments32 + 1) & 1u, &sm.abort, kItemLimitNs));
                 if (!ok) break;
                 Segment32 g;
                 g.n = 0;  // the end

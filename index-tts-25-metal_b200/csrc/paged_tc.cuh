@@ -30,16 +30,22 @@ __device__ __forceinline__ bool mbar_try(unsigned long long* bar, uint32_t parit
         : "memory");
     return done != 0;
 }
+// Limit of a wait that lasts as long as the work on an item: 2^30 keys take a CTA
+// up to a minute.  The roles that do the work wait for each unit with the limit
+// above and raise the abort flag, which ends this wait, too.
+constexpr unsigned long long kItemLimitNs = 120 * 1000000000ull;
+
 // Waits for a phase of `bar`.  Gives up when the time limit passes (and raises
 // the CTA's abort flag) or, if `abort` is given, when another role has raised it.
-__device__ __forceinline__ bool mbar_wait(unsigned long long* bar, uint32_t parity, int* abort) {
+__device__ __forceinline__ bool mbar_wait(unsigned long long* bar, uint32_t parity, int* abort,
+                                          unsigned long long limit = kWaitLimitNs) {
     if (mbar_try(bar, parity)) return true;
     const unsigned long long t0 = globaltimer_ns();
     for (uint32_t i = 0;; ++i) {
         if (mbar_try(bar, parity)) return true;
         if ((i & 15u) == 15u) {
             if (abort && *reinterpret_cast<volatile int*>(abort)) return false;
-            if (globaltimer_ns() - t0 > kWaitLimitNs) {
+            if (globaltimer_ns() - t0 > limit) {
                 if (abort) *reinterpret_cast<volatile int*>(abort) = 1;
                 return false;
             }

@@ -669,3 +669,16 @@ def test_attention_without_measure_is_not_begun(paged, max_fresh, dtype):
     table = torch.full((1, 2 ** 30 // bs), -1, dtype=torch.int32, device=DEV)
     paged.attention(q, cache, cache, table, ints([2 ** 30]), ints([0, rows]), max_fresh, out=out)
     assert (out == 3).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_items_of_seconds(paged, dtype):
+    """Items that take their CTA longer (3 and 4 s) than a wait for a unit may; their keys are one block, repeated."""
+    heads, dim, bs = 148, 128, 128
+    keys, fresh = (2 ** 26, 128) if dtype == F32 else (2 ** 28, 256)
+    k = torch.zeros(1, bs, heads, dim, dtype=dtype, device=DEV)
+    v = torch.zeros(1, bs, heads, dim, dtype=dtype, device=DEV)
+    q = torch.ones(fresh, heads, dim, dtype=dtype, device=DEV)
+    table = torch.zeros(1, keys // bs, dtype=torch.int32, device=DEV)
+    out = paged.attention(q, k, v, table, ints([keys]), ints([0, fresh]), fresh)
+    assert (out == 0).all()
