@@ -69,6 +69,10 @@ static_assert(2 * kSoftmaxRegs + kOtherRegs == 3 * kRegsLaunch && kSoftmaxRegs >
 constexpr int kTileCtas = 148;
 constexpr int kTileItem = 1;  // what an item costs besides its units, in units
 constexpr float kGrow = 8.f;  // log2 of the growth of the maximum that is let pass
+// Keys over which tensor memory sums up an item's output.  The tensor core's accumulation does not round to nearest:
+// with 2^20 keys at a stretch the result came out 6e-3 short, with 2^14 1e-4.  Then the sums so far go to the item's
+// slot of the workspace, where they are added up in fp32 (148 items of 2^17 keys 2.12 ms at a stretch, 2.18 ms so).
+constexpr int kStretch = 1 << 14;
 
 // A part of an item in this share: units [k0, k0 + n) of the item.
 struct Segment {
@@ -203,6 +207,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     using Smem = TileSmem<D>;
     Smem& sm = *reinterpret_cast<Smem*>(smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023));
     constexpr int NS = Smem::kStages, kHalves = Smem::kHalves, KU = kUnitOf<D>, NC = KU / 32;
+    constexpr int kFold = kStretch / KU;  // units
     constexpr uint32_t kTileBytes = Smem::kTileBytes, kHalfBytes = kTileBytes / kHalves;
     constexpr uint32_t kQHalf = Smem::kQBytes / kHalves;
     constexpr uint32_t kP = 2 * KU, kO = 3 * KU;  // columns of tensor memory: S of tile t at KU t, P at kP + KU / 2 t, O at kO + D t
@@ -368,7 +373,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 if (!wait(&sm.p_ready[t], ph_p)) break;  // after which the unit's scores are read, too
                 ph_p ^= 1u;
                 tc_after();
-                if (elect()) output(xv, j > 0);
+                if (elect()) output(xv, (j & (kFold - 1)) != 0);
                 __syncwarp();
             }
             for (int j = units; j < gn && ok; ++j) {  // units that none of the tile's rows sees
@@ -469,6 +474,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             if (row < g.rows) seen = min(max(g.pos + over_group(a, g.first + row) + 1, 0), a.cap) - g.k0 * KU;
             else seen = -g.k0 * KU;
             float m = -INFINITY, l = 0.f;
+            // The item's slot (where it lies in this share alone: the one that a later item may take): earlier sums.
+            const auto kept = [&] { return part_slot<kTileRows, D>(a, blockIdx.x, g.parts == 1 ? 0 : 1) + (size_t)row * D; };
+            const auto kept_ml = [&] {
+                return reinterpret_cast<float2*>(part_slot<kTileRows, D>(a, blockIdx.x, g.parts == 1 ? 0 : 1) + kTileRows * D) + row;
+            };
+            const auto since = [&](float then) { return then == m ? 1.f : ex2(then - m); };  // both may be -inf
             for (int j = 0; j < units; ++j, seen -= KU) {
                 ok = mbar_wait(&sm.s_ready[t], ph_s, &sm.abort);
                 ok = __all_sync(0xffffffffu, ok);
@@ -520,13 +531,36 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     ph_o ^= 1u;
                     if (!ok) break;
                     tc_after();
+                    if (__builtin_expect((j & (kFold - 1)) == 0, 0)) {
+                        const float2 old = j == kFold ? make_float2(m, 0.f) : *kept_ml();
+                        const float f = since(old.x);
+#pragma unroll 1
+                        for (int c = 0; c < D / 16; ++c) {
+                            uint32_t o[16];
+                            tmem_ld16(o_col + 16u * c, o);
+                            tc_wait_ld(o);
+                            float4* to = reinterpret_cast<float4*>(kept() + 16 * c);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                float4 y = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
+                                                       __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
+                                if (j > kFold) {
+                                    const float4 z = to[e];
+                                    y = make_float4(fmaf(z.x, f, y.x), fmaf(z.y, f, y.y), fmaf(z.z, f, y.z), fmaf(z.w, f, y.w));
+                                }
+                                to[e] = y;
+                            }
+                        }
+                        *kept_ml() = make_float2(m, fmaf(old.y, f, l));
+                        l = 0.f;
+                    }
                 }
                 const bool grow = top > m + kGrow || (m == -INFINITY && top > m);
                 if (__any_sync(0xffffffffu, grow)) {
                     const float mn = fmaxf(m, top), f = mn == -INFINITY ? 1.f : ex2(m - mn);
                     m = mn;
                     l *= f;
-                    if (j > 0) {
+                    if (j & (kFold - 1)) {
 #pragma unroll
                         for (int c = 0; c < D / 16; ++c) {
                             uint32_t o[16];
@@ -575,6 +609,22 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             float* slot = whole ? nullptr : part_slot<kTileRows, D>(a, blockIdx.x, g.parts > 1 ? 1 : 0);
             T* dst = live && whole ? out_row<T>(a, g.start, g.first, row, g.kvh) : nullptr;
             if (!ok) break;
+            if (__builtin_expect(units > kFold, 0)) {  // the earlier sums join
+                const float2 old = *kept_ml();
+                const float f = since(old.x);
+                l = fmaf(old.y, f, l);
+#pragma unroll 1
+                for (int c = 0; c < D / 16; ++c) {
+                    uint32_t o[16];
+                    tmem_ld16(o_col + 16u * c, o);
+                    tc_wait_ld(o);
+                    const float* z = kept() + 16 * c;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(fmaf(z[e], f, __uint_as_float(o[e])));
+                    tmem_st16(o_col + 16u * c, o);
+                }
+                tc_wait_st();
+            }
             const float inv = l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) {

@@ -682,3 +682,30 @@ def test_attention_items_of_seconds(paged, dtype):
     table = torch.zeros(1, keys // bs, dtype=torch.int32, device=DEV)
     out = paged.attention(q, k, v, table, ints([keys]), ints([0, fresh]), fresh)
     assert (out == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("fresh,dim,split", [(1, 128, False), (8, 64, False), (300, 128, False), (260, 64, False), (300, 128, True)])
+@pytest.mark.parametrize("lift", [False, True])
+def test_attention_long_sums(paged, fresh, dim, split, lift, dtype):
+    """The mean of values that are all 1, over 2^19 + 77 keys, is 1, whether an item lies in one CTA or in many, and
+    with the largest scores at the end (every sum before is scaled) or anywhere.
+
+    Half a step of the type for the weights, which the products take rounded while their sum is not, and half a step
+    for the output.  The sums: a step of 2^-23 of the sum for each 16 keys of at most 2^14 at a stretch (2^10 2^-23),
+    2^-24 for each of the up to 2^5 stretches, and for a row's sum of weights the same for each 64 keys of a stretch;
+    with 16 keys at a time, 2^15 sums to the nearest, whose errors of 2^-24 have either sign: 2^-24 2^7.5 and ten
+    times that."""
+    n, bs, requests = 2 ** 19 + 77, 128, 2 if split else 300
+    g = torch.Generator(device=DEV).manual_seed(fresh + dim)
+    blocks = (n + bs - 1) // bs
+    k = torch.randn(blocks, bs, 1, dim, generator=g, device=DEV)
+    q = torch.randn(fresh * requests, 1, dim, generator=g, device=DEV)
+    if lift:
+        q[:, :, 0] = 4.0
+        k[-1, :, :, 0] = 12.0 * dim ** 0.5 / 8
+    v = torch.ones(blocks, bs, 1, dim, dtype=dtype, device=DEV)
+    table = torch.arange(blocks, dtype=torch.int32, device=DEV).expand(requests, blocks).contiguous()
+    out = paged.attention(q.to(dtype), k.to(dtype), v, table, ints([n] * requests),
+                          ints([fresh * b for b in range(requests + 1)]), fresh)
+    assert (out.double() - 1).abs().max() <= torch.finfo(dtype).eps + 2 ** -13 + 2 ** -18
