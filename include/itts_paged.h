@@ -89,7 +89,9 @@ typedef struct itts_paged_tables_args {
 int itts_paged_tables(int device, const itts_paged_tables_args* args, void* stream);
 
 /* A paged cache: K and V of [blocks][block_size][heads][head_dim] elements at
- * any strides (in elements; head_dim contiguous). */
+ * any strides (in elements; head_dim contiguous).  A stride of 0 repeats a
+ * dimension, such as one head for all: the attention reads it, the append
+ * refuses it. */
 typedef struct itts_paged_cache {
     void* k;
     void* v;
@@ -153,7 +155,7 @@ typedef struct itts_paged_attention_args {
     int32_t q_heads; /* a multiple of cache.heads, at most 128 times it */
     int32_t rows;    /* 0 .. 2^30, and so is rows * q_heads / heads */
     int64_t q_row_stride, q_head_stride; /* elements */
-    int64_t out_row_stride, out_head_stride;
+    int64_t out_row_stride, out_head_stride; /* not 0 */
     const int32_t* q_start; /* [requests + 1] */
     const int32_t* lens;    /* [requests] */
     const int32_t* table;   /* [requests][max_blocks] */

@@ -131,6 +131,10 @@ int itts_paged_append(int device, const itts_paged_append_args* a, void* stream)
         if (a->rows == 0) return;
         check(a->k && a->v && a->slots, "null argument");
         const int64_t size = size_of(a->source_type), most = (int64_t(1) << 40) / size;
+        const itts_paged_cache& c = a->cache;
+        check(c.k_token_stride && c.v_token_stride && (c.blocks == 1 || (c.k_block_stride && c.v_block_stride)) &&
+                  (c.heads == 1 || (c.k_head_stride && c.v_head_stride)),
+              "paged cache repeats a dimension that the append writes");
         check(aligned(a->k, size_t(size)) && aligned(a->v, size_t(size)), "key or value rows are misaligned");
         for (int64_t s : {a->k_row_stride, a->k_head_stride, a->v_row_stride, a->v_head_stride})
             check(s >= 0 && s < most, "key or value stride out of range");
@@ -164,6 +168,7 @@ int itts_paged_attention(int device, const itts_paged_attention_args* a, void* s
                   stride16(a->q_head_stride, a->cache.type) && stride16(a->out_row_stride, a->cache.type) &&
                   stride16(a->out_head_stride, a->cache.type),
               "q and out addresses and strides must be multiples of 16 bytes");
+        check((a->rows == 1 || a->out_row_stride) && (a->q_heads == 1 || a->out_head_stride), "out repeats a dimension");
         OnDevice on(device);
         ck(itts::paged::launch_attention(*a, static_cast<cudaStream_t>(stream)), "paged attention");
     });

@@ -702,6 +702,11 @@ cudaError_t make_block_map(CUtensorMap* map, const itts_paged_cache& c, bool v, 
     const int size = c.type == ITTS_PAGED_F32 ? 4 : 2;
     // the stride of a dimension of one is never used, but has to be a legal one
     const auto bytes = [&](long long stride, int n) { return n == 1 ? 16ull : (unsigned long long)(stride * size); };
+    // a map does not repeat a dimension
+    const auto repeats = [](long long stride, int n) { return n > 1 && stride == 0; };
+    if (repeats(v ? c.v_token_stride : c.k_token_stride, c.block_size) ||
+        repeats(v ? c.v_head_stride : c.k_head_stride, c.heads) || repeats(v ? c.v_block_stride : c.k_block_stride, c.blocks))
+        return cudaErrorNotSupported;
     const cuuint64_t dims[4] = {cuuint64_t(c.head_dim), cuuint64_t(c.block_size), cuuint64_t(c.heads), cuuint64_t(c.blocks)};
     const cuuint64_t strides[3] = {bytes(v ? c.v_token_stride : c.k_token_stride, c.block_size),
                                    bytes(v ? c.v_head_stride : c.k_head_stride, c.heads),
@@ -722,6 +727,7 @@ cudaError_t make_row_map(CUtensorMap* map, const Attn& a, int tokens) {
     const auto fn = encode();
     if (!fn) return cudaErrorNotSupported;
     const int heads = a.group * a.c.heads;
+    if ((heads > 1 && a.q_head == 0) || (a.rows > 1 && a.q_row == 0)) return cudaErrorNotSupported;
     const cuuint64_t dims[3] = {cuuint64_t(a.c.head_dim), cuuint64_t(heads), cuuint64_t(a.rows)};
     const cuuint64_t strides[2] = {heads == 1 ? 16ull : cuuint64_t(a.q_head * 2), a.rows == 1 ? 16ull : cuuint64_t(a.q_row * 2)};
     const cuuint32_t box[3] = {64, cuuint32_t(a.group), cuuint32_t(tokens)}, one[3] = {1, 1, 1};

@@ -709,3 +709,30 @@ def test_attention_long_sums(paged, fresh, dim, split, lift, dtype):
     out = paged.attention(q.to(dtype), k.to(dtype), v, table, ints([n] * requests),
                           ints([fresh * b for b in range(requests + 1)]), fresh)
     assert (out.double() - 1).abs().max() <= torch.finfo(dtype).eps + 2 ** -13 + 2 ** -18
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("fresh", [1, 7, 200])
+@pytest.mark.parametrize("what", ["heads", "tokens", "blocks", "rows", "query heads"])
+def test_attention_reads_repeated_dimensions(paged, what, fresh, dtype):
+    """Strides of 0 (expanded tensors) give what their copies give; within an allowance for another kernel's order."""
+    g = torch.Generator(device=DEV).manual_seed(fresh)
+    r = lambda *shape: torch.randn(*shape, generator=g, device=DEV).to(dtype)
+    k, v, q = r(12, 32, 4, 64), r(12, 32, 4, 64), r(2 * fresh, 8, 64)
+    if what == "heads":
+        k, v = k[:, :, :1].expand(12, 32, 4, 64), v[:, :, 1:2].expand(12, 32, 4, 64)
+    elif what == "tokens":
+        k, v = k[:, :1].expand(12, 32, 4, 64), v[:, 5:6].expand(12, 32, 4, 64)
+    elif what == "blocks":
+        k, v = k[:1].expand(12, 32, 4, 64), v[3:4].expand(12, 32, 4, 64)
+    elif what == "rows":
+        q = q[:1].expand(2 * fresh, 8, 64)
+    else:
+        q = q[:, :1].expand(2 * fresh, 8, 64)
+    table = ints([[0, 1, 2, 3, 4, 5, 6], [7, 8, 9, 10, 11, 0, 1]])
+    rest = (table, ints([210, 201]), ints([0, fresh, 2 * fresh]), fresh)
+    got = paged.attention(q, k, v, *rest).double()
+    want = paged.attention(q.contiguous(), k.contiguous(), v.contiguous(), *rest).double()
+    # both round weights and output to the type (half a step each); sums of 210 terms in fp32 otherwise
+    top = v.double().abs().max()
+    assert (got - want).abs().max() <= top * (2 * torch.finfo(dtype).eps + 210 * 2 ** -24)

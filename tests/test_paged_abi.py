@@ -194,3 +194,18 @@ def test_python_binding_refuses_host_tensors(gpt_mod, paged):
         paged.attention(x, c, c, i[None], i, i, 1)
     with pytest.raises(ValueError, match="CUDA tensor"):
         paged.tables(i, i, i[None], i, i, 16, lens=i, q_start=i, positions=i, slots=i, status=i)
+
+
+@pytest.mark.parametrize("field", ["k_block_stride", "k_token_stride", "k_head_stride", "v_block_stride", "v_token_stride",
+                                   "v_head_stride"])
+def test_append_refuses_a_repeated_dimension(lib, gpt_mod, paged, field):
+    a = append(paged)
+    setattr(a.cache, field, 0)
+    refused(lib, gpt_mod, "itts_paged_append", a, "repeats a dimension")
+
+
+@pytest.mark.parametrize("field", ["out_row_stride", "out_head_stride"])
+def test_attention_refuses_a_repeated_output(lib, gpt_mod, paged, field):
+    a = attention(paged)
+    setattr(a, field, 0)
+    refused(lib, gpt_mod, "itts_paged_attention", a, "out repeats a dimension")
