@@ -736,3 +736,39 @@ def test_attention_reads_repeated_dimensions(paged, what, fresh, dtype):
     # both round weights and output to the type (half a step each); sums of 210 terms in fp32 otherwise
     top = v.double().abs().max()
     assert (got - want).abs().max() <= top * (2 * torch.finfo(dtype).eps + 210 * 2 ** -24)
+
+
+def test_threads_with_their_own_streams(paged):
+    """Four threads at once, each with its stream, type and shape, give what each gives alone."""
+    import threading
+    steps = [Step([(1, 500)] * 40, 16, 8, 128, bs=64, dtype=BF16, seed=1), Step(MIXES["chunks"], dtype=F32, seed=2),
+             Step(MIXES["chunks"], 16, 8, 128, bs=128, dtype=F16, seed=3), Step(MIXES["few"], dtype=F32, seed=4)]
+    alone = [s.run(paged).clone() for s in steps]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(50):
+                    out = torch.empty_like(steps[i].q)
+                    paged.attention(steps[i].q, steps[i].kc, steps[i].vc, steps[i].table, steps[i].lens,
+                                    steps[i].q_start, max(steps[i].fresh), out=out)
+                    if not torch.equal(out[:steps[i].start[-1]], alone[i][:steps[i].start[-1]]):
+                        failed.append(i)
+                try:
+                    paged.attention(steps[i].q, steps[i].kc, steps[i].vc, steps[i].table, steps[i].lens,
+                                    steps[i].q_start, 0)
+                except ValueError as e:  # each thread has its own message
+                    if "max_fresh" not in str(e):
+                        failed.append(str(e))
+        except Exception as e:  # noqa: BLE001
+            failed.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
