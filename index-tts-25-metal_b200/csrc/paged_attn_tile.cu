@@ -139,6 +139,10 @@ __device__ __forceinline__ uint32_t pack16<__nv_bfloat16>(float x, float y) {
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -426,21 +430,24 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                                      g.start + over_group(a, row0), &sm.q_full[t]);
                     }
                 } else {
-                    const uint32_t flip = a.sign < 0.f ? 0x80008000u : 0u;
                     constexpr int kChunks = D / 8;
+                    const auto chunk = [&](int r, int ch) {
+                        return sm.q[t] + (ch / 8) * kQHalf + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
+                    };
 #pragma unroll 4
-                    for (int y = lane; y < 128 * kChunks; y += 32) {
+                    for (int y = lane; y < 128 * kChunks; y += 32) {  // all in flight at once: four at a time took 6 us a tile
                         const int r = y / kChunks, ch = y % kChunks;
-                        uint4 v = make_uint4(0, 0, 0, 0);
-                        if (128 * t + r < g.rows) {
-                            const int tok = over_group(a, row0 + r), hd = (row0 + r) - tok * a.group;
-                            v = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) +
-                                                                     (long long)(g.start + tok) * a.q_row +
-                                                                     (long long)(g.kvh * a.group + hd) * a.q_head) + ch);
-                            v = make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
-                        }
-                        *reinterpret_cast<uint4*>(sm.q[t] + (ch / 8) * kQHalf + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = v;
+                        const bool live = 128 * t + r < g.rows;
+                        const int tok = over_group(a, row0 + (live ? r : 0)), hd = row0 + (live ? r : 0) - tok * a.group;
+                        cp16(smem_u32(chunk(r, ch)), static_cast<const T*>(a.q) + (long long)(g.start + tok) * a.q_row +
+                                                         (long long)(g.kvh * a.group + hd) * a.q_head + 8 * ch, live ? 16 : 0);
                     }
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    if (a.sign < 0.f)
+                        for (int y = lane; y < 128 * kChunks; y += 32) {  // this lane's own
+                            uint4& v = *reinterpret_cast<uint4*>(chunk(y / kChunks, y % kChunks));
+                            v = make_uint4(v.x ^ 0x80008000u, v.y ^ 0x80008000u, v.z ^ 0x80008000u, v.w ^ 0x80008000u);
+                        }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sm.q_full[t]);
