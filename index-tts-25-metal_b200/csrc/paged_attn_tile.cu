@@ -34,7 +34,7 @@
 //   warp 10         walks the items ahead of the others, publishes their extents in
 //                   shared memory and loads Q of the tiles as soon as the last
 //                   scores with the one before are done (TMA where the query
-//                   heads of a group divide a tile, plain loads otherwise).
+//                   heads of a group divide a tile, cp.async otherwise).
 // Tensor memory: S of the tiles, P of the tiles, O of the tiles.
 //
 // P is rounded to the 16-bit type once (V's type: the products take one type);
