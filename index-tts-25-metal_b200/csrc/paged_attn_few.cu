@@ -47,6 +47,11 @@ constexpr int kSimtMost = 8;   // rows of 32 bits that the CUDA cores take
 constexpr int kFewWarps = 4;
 constexpr int kFewThreads = 32 * kFewWarps;
 constexpr int kRingBytes = 24 * 1024;  // per warp
+// Units over which a warp's sums run on.  A weight below 2^-24 of a running fp32 sum is lost to it, and every sum is
+// off by up to that much: over 2^19 keys, 2^17 of a warp, with one key 17 nats ahead, fp32 results were off by 4e-3
+// (2e-5 so).  After a stretch the warps' sums meet in the item's slot of the workspace, as at the end of a share: 2^-16
+// for the stretch and 2^-24 for each.  Us without and with: 16 steps over 420 keys 12.2 / 12.4, 64 over 16384 322 / 324.
+constexpr int kFewStretch = 256;
 
 template <class T, int D>
 struct Few {
@@ -314,10 +319,13 @@ struct Rows {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                sc[t][e] = ex2(fmaf(sc[t][e], scale2, -ref[e >> 1]));
-                l[e >> 1] += sc[t][e];
-            }
+            for (int e = 0; e < 4; ++e) sc[t][e] = ex2(fmaf(sc[t][e], scale2, -ref[e >> 1]));
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            float sum = sc[0][2 * j] + sc[0][2 * j + 1];
+            if constexpr (NT == 2) sum += sc[1][2 * j] + sc[1][2 * j + 1];
+            l[j] += sum;
+        }
 
         if constexpr (sizeof(T) == 2) {
             uint32_t ph[4], pl[4];
@@ -470,17 +478,24 @@ struct Rows32 {
             }
         }
         const int half = D == 128 ? 0 : lane & 16;
+        float4 y[R];  // of this sub-block, added to the running sums at once
 #pragma unroll
         for (int i = 0; i < kIter; ++i) {
             const float4 x = v[32 * i];
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 const float p = __shfl_sync(0xffffffffu, s[r % kE], half + 4 * i + lane_of(r));
-                const float2 y = fma2(make_float2(p, p), make_float2(x.x, x.y), make_float2(o[r].x, o[r].y));
-                const float2 z = fma2(make_float2(p, p), make_float2(x.z, x.w), make_float2(o[r].z, o[r].w));
-                o[r] = make_float4(y.x, y.y, z.x, z.y);
+                if (i == 0) {
+                    y[r] = make_float4(p * x.x, p * x.y, p * x.z, p * x.w);
+                } else {
+                    const float2 a = fma2(make_float2(p, p), make_float2(x.x, x.y), make_float2(y[r].x, y[r].y));
+                    const float2 b = fma2(make_float2(p, p), make_float2(x.z, x.w), make_float2(y[r].z, y[r].w));
+                    y[r] = make_float4(a.x, a.y, b.x, b.y);
+                }
             }
         }
+#pragma unroll
+        for (int r = 0; r < R; ++r) o[r] = make_float4(o[r].x + y[r].x, o[r].y + y[r].y, o[r].z + y[r].z, o[r].w + y[r].w);
     }
     __device__ __forceinline__ void end(float* dst, float2* ml, int rows, int lane) {
 #pragma unroll
@@ -517,7 +532,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_attn_few(const __grid_consta
     using Math = Rows<T, D, R>;
     extern __shared__ __align__(128) unsigned char ring[];
     __shared__ PlanSmem<kFewThreads> plan_smem;
-    __shared__ float2 ml[kFewWarps][R];
+    __shared__ float2 ml[kFewWarps][R], kept[2][R];
     constexpr int S = F::kStages, KS = F::kKeys;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     unsigned char* my_ring = ring + warp * kRingBytes;
@@ -578,9 +593,11 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_attn_few(const __grid_consta
 
     Math math;
     int rows = 0, first = 0;
+    int stretch = 0, folds = 0;         // units of this stretch of the item, stretches before it
     bool fresh = false, begun = false;  // begun: the item's first unit is this share's
-    const auto begin = [&] {            // the item that the arithmetic has come to
-        begun = at.k == 0;
+    const auto begin = [&] {            // the item that the arithmetic has come to, or its next stretch
+        if (folds == 0) begun = at.k == 0;
+        stretch = 0;
         first = at.t * R;
         rows = min(R, at.r.rows - first);
         math.begin(
@@ -606,24 +623,27 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_attn_few(const __grid_consta
 
         math.unit(my_ring + s * (2 * F::kHalf), ring_u + s * (2 * F::kHalf), key0, named, a.scale2, lane);
 
-        if (at.k + 1 < at.nk && i + 1 < n) {
+        const bool last = at.k + 1 == at.nk || i + 1 == n;
+        if (__builtin_expect(!last && ++stretch < kFewStretch, 1)) {
             at.advance(a, 1);
             continue;
         }
 
-        // The item's keys end here, or this share does: the warps' sums meet.
+        // The item's keys end here, or this share or a stretch does: the warps' sums meet.
         // Each warp's output goes to the stage it has just consumed.
         float* mine = reinterpret_cast<float*>(my_ring + s * (2 * F::kHalf));
         __syncwarp();
         math.end(mine, ml[warp], rows, lane);
         __syncthreads();
-        const bool whole = begun && at.k + 1 == at.nk;
-        float* slot = whole ? nullptr : part_slot<R, D>(a, blockIdx.x, begun ? 1 : 0);
+        const bool whole = last && begun && at.k + 1 == at.nk;
+        float* slot = part_slot<R, D>(a, blockIdx.x, begun ? 1 : 0);
         for (int x = threadIdx.x; x < rows * (D / 4); x += kFewThreads) {
             const int r = x / (D / 4), d4 = x % (D / 4);
             float M = -INFINITY, L = 0.f;
 #pragma unroll
             for (int w = 0; w < kFewWarps; ++w) M = fmaxf(M, ml[w][r].x);
+            float2 old = make_float2(-INFINITY, 0.f);
+            if (__builtin_expect(folds > 0, 0)) M = fmaxf(M, (old = kept[folds & 1][r]).x);
             const float rf = M == -INFINITY ? 0.f : M;
             float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
@@ -634,20 +654,27 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_attn_few(const __grid_consta
                 L += ml[w][r].y * f;
                 y = make_float4(y.x + v.x * f, y.y + v.y * f, y.z + v.z * f, y.w + v.w * f);
             }
+            if (__builtin_expect(folds > 0, 0)) {  // written by this thread at the stretch before
+                const float f = ex2(old.x - rf);
+                const float4 v = *reinterpret_cast<const float4*>(slot + r * D + 4 * d4);
+                L += old.y * f;
+                y = make_float4(y.x + v.x * f, y.y + v.y * f, y.z + v.z * f, y.w + v.w * f);
+            }
             if (whole) {
                 store4<T>(out_row<T>(a, at.r.start, first, r, at.h) + 4 * d4, normalised(y, L));
             } else {
                 *reinterpret_cast<float4*>(slot + r * D + 4 * d4) = y;
-                if (d4 == 0) reinterpret_cast<float2*>(slot + R * D)[r] = make_float2(M, L);
+                if (d4 == 0) (last ? reinterpret_cast<float2*>(slot + R * D) : kept[(folds + 1) & 1])[r] = make_float2(M, L);
             }
         }
-        if (!whole && begun && threadIdx.x == 0) {  // it goes on: in how many shares
-            const int last = cta_of(sh, sh.u0 + i + (at.nk - at.k) - 1);
-            put_record(a, blockIdx.x, last - int(blockIdx.x) + 1, at.h, rows, at.r.start, first);
+        if (last && !whole && begun && threadIdx.x == 0) {  // it goes on: in how many shares
+            const int end = cta_of(sh, sh.u0 + i + (at.nk - at.k) - 1);
+            put_record(a, blockIdx.x, end - int(blockIdx.x) + 1, at.h, rows, at.r.start, first);
         }
         __syncthreads();
         at.advance(a, 1);
         fresh = true;
+        folds = last ? 0 : folds + 1;
     }
 }
 

@@ -1,0 +1,50 @@
+"""The paged attention at the ends of its numeric ranges, on a B200: weights far
+below the largest, against the definition in 64 bits."""
+import importlib
+import math
+
+import pytest
+import torch
+
+from test_gpu_paged import DEV, F32, ints
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def paged():
+    return importlib.import_module("index-tts-25-metal_b200.paged")
+
+
+def one_key_ahead(paged, dtype, n, fresh, dim, requests, lead, top, value):
+    """Attention over n keys of equal scores but for key `top`, which is `lead` nats ahead and has the value `value`
+    where the others have 1.  Returns the output and, per row, what it should be."""
+    bs = 128
+    blocks = (n + bs - 1) // bs
+    k = torch.zeros(blocks * bs, 1, dim, dtype=dtype, device=DEV)
+    v = torch.ones_like(k)
+    k[top, 0, 0], v[top] = lead, value
+    q = torch.zeros(fresh * requests, 1, dim, dtype=dtype, device=DEV)
+    q[:, 0, 0] = 1.0
+    table = torch.arange(blocks, dtype=torch.int32, device=DEV).expand(requests, blocks).contiguous()
+    out = paged.attention(q, k.view(blocks, bs, 1, dim), v.view(blocks, bs, 1, dim), table, ints([n] * requests),
+                          ints([fresh * b for b in range(requests + 1)]), fresh, scale=1.0)
+    others = torch.arange(n - fresh, n, dtype=torch.float64, device=DEV)  # equal keys that a row sees
+    tail = others * math.exp(-float(k[top, 0, 0]))
+    return out.double().view(requests, fresh, dim), ((value + tail) / (1 + tail))[None, :, None]
+
+
+@pytest.mark.parametrize("fresh,dim,requests", [(1, 128, 300), (1, 64, 150), (2, 128, 150), (8, 64, 150), (16, 128, 150)])
+@pytest.mark.parametrize("value", [0.0, 1.0])
+def test_attention_fp32_sums_over_many_keys(paged, value, fresh, dim, requests):
+    """Items of 2^19 keys in one CTA, one key so far ahead that each other one is below half a step of a sum that holds
+    it.  For the sums above and below the line: 2^8 additions of units at a stretch and 2^6 of stretches (2^-16 and
+    2^-18), 2^-18 within a unit of up to 64 keys (24 accumulations of the tensor core, not to the nearest, 2^-23 each,
+    and less on the CUDA cores); the exponent, up to 2^5 in size, 2^-24 of it from each of two roundings and 2^-22 from
+    the exponential itself: 2^-17."""
+    n = 2 ** 19 + 77
+    for lead in (17.2, 17.35):
+        for top in (0, n - fresh):
+            got, want = one_key_ahead(paged, F32, n, fresh, dim, requests, lead, top, value)
+            tol = want * (2 * (2.0 ** -16 + 2.0 ** -18 + 2.0 ** -18) + 2.0 ** -17 + 2.0 ** -24)
+            assert bool(((got - want).abs() <= tol).all()), float((got / want - 1).abs().max())
