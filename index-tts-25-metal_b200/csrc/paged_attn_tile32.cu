@@ -49,11 +49,17 @@ static_assert(kRegsSoftmax + kRegsOut + 2 * kRegsSplit + kRegsIssue == 5 * kRegs
 static_assert(kRegsSoftmax >= kRegsLaunch && kRegsOut >= kRegsLaunch, "setmaxnreg.inc does not lower");
 static_assert(kRegsSplit <= kRegsLaunch && kRegsIssue <= kRegsLaunch, "setmaxnreg.dec does not raise");
 constexpr int kSegments32 = 4;
+// Units of a segment at most: a stretch over which a row's sums run on.  Every addition is off by up to 2^-24 of the
+// sum, one way if the addends are alike: over 2^19 keys, one of them 17 nats ahead, the others' share came out 2.5e-4
+// wrong (1.1e-5 so).  A longer part of an item is several segments, whose sums meet in the item's slot of the workspace;
+// each loads Q again (20 requests of 60 rows over 20000 keys 1.23 ms either way).
+constexpr int kStretch32 = 256;
 
 struct Segment32 {
     int first, rows, k0, n;  // first row of the item in its request, its rows (<= 128), first unit, units
     int start, pos, kvh;     // first row of the request, position of its row 0, kv head
     int parts;               // 0: begins and ends here; 1: goes on from another share; n > 1: begins here, n shares
+    bool later, more;        // segments of the item in this share come before, come after it
 };
 
 // Where the keys of a unit lie.
@@ -95,6 +101,7 @@ __device__ __forceinline__ Segment32 segment32(const Attn& a, const Walk32& w, c
     s.pos = w.r.len - w.r.tokens;
     s.kvh = w.h;
     s.parts = w.parts(sh);
+    s.later = s.more = false;
     return s;
 }
 
@@ -366,7 +373,22 @@ __global__ void __launch_bounds__(kThreads32, 1) k_attn_tile32(const __grid_cons
             }
             if (!ok) break;
             if (row < g.rows) {
-                if (g.parts == 0) {
+                // the item's slot (where it lies in this share alone: the one that a later item may take)
+                float* slot = part_slot<kRows32, D>(a, blockIdx.x, g.parts == 1 ? 0 : 1);
+                if (g.later) {
+                    const float2 old = reinterpret_cast<const float2*>(slot + kRows32 * D)[row];
+                    const float m = fmaxf(old.x, ml.x), f = old.x == m ? 1.f : ex2(old.x - m), e = ml.x == m ? 1.f : ex2(ml.x - m);
+                    ml = make_float2(m, fmaf(old.y, f, ml.y * e));
+#pragma unroll
+                    for (int c = 0; c < D; c += 4) {
+                        const float4 z = *reinterpret_cast<const float4*>(slot + (size_t)row * D + c);
+                        o[c] = fmaf(z.x, f, o[c] * e);
+                        o[c + 1] = fmaf(z.y, f, o[c + 1] * e);
+                        o[c + 2] = fmaf(z.z, f, o[c + 2] * e);
+                        o[c + 3] = fmaf(z.w, f, o[c + 3] * e);
+                    }
+                }
+                if (g.parts == 0 && !g.more) {
                     float* dst = out_row<float>(a, g.start, g.first, row, g.kvh);
                     const float inv = ml.y == 0.f ? 0.f : 1.0f / ml.y;
 #pragma unroll
@@ -375,7 +397,6 @@ __global__ void __launch_bounds__(kThreads32, 1) k_attn_tile32(const __grid_cons
                             ml.y == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
                                         : make_float4(o[c] * inv, o[c + 1] * inv, o[c + 2] * inv, o[c + 3] * inv);
                 } else {
-                    float* slot = part_slot<kRows32, D>(a, blockIdx.x, g.parts > 1 ? 1 : 0);
 #pragma unroll
                     for (int c = 0; c < D; c += 4)
                         *reinterpret_cast<float4*>(slot + (size_t)row * D + c) = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
@@ -515,14 +536,22 @@ __global__ void __launch_bounds__(kThreads32, 1) k_attn_tile32(const __grid_cons
             // ---- items
             Walk32 w;
             w.start(a, sh);
-            bool ok = true;
+            bool ok = true, later = false;
+            int parts = 0;  // of the item, as its first segment has it
             for (int x = 0;; ++x) {
                 if (x >= kSegments32)
                     ok = uniform(mbar_wait(&sm.seg_empty[x % kSegments32], uint32_t(x / kSegments32 + 1) & 1u, &sm.abort, kItemLimitNs));
                 if (!ok) break;
                 Segment32 g;
                 g.n = 0;  // the end
-                if (w.work()) g = segment32(a, w, sh);
+                if (w.work()) {
+                    g = segment32(a, w, sh);
+                    if (later) g.parts = parts;
+                    parts = g.parts;
+                    g.later = later;
+                    g.more = later = g.n > kStretch32;
+                    g.n = min(g.n, kStretch32);
+                }
                 if (lane == 0) {
                     sm.seg[x % kSegments32] = g;
                     mbar_arrive(&sm.seg_full[x % kSegments32]);

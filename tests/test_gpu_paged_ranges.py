@@ -34,7 +34,8 @@ def one_key_ahead(paged, dtype, n, fresh, dim, requests, lead, top, value):
     return out.double().view(requests, fresh, dim), ((value + tail) / (1 + tail))[None, :, None]
 
 
-@pytest.mark.parametrize("fresh,dim,requests", [(1, 128, 300), (1, 64, 150), (2, 128, 150), (8, 64, 150), (16, 128, 150)])
+@pytest.mark.parametrize("fresh,dim,requests", [(1, 128, 300), (1, 64, 150), (2, 128, 150), (8, 64, 150), (16, 128, 150),
+                                                (300, 128, 160), (129, 64, 160)])
 @pytest.mark.parametrize("value", [0.0, 1.0])
 def test_attention_fp32_sums_over_many_keys(paged, value, fresh, dim, requests):
     """Items of 2^19 keys in one CTA, one key so far ahead that each other one is below half a step of a sum that holds
