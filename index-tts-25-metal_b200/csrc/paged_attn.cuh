@@ -23,6 +23,7 @@
 #include <cuda_fp16.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "common.cuh"
 #include "paged.hpp"
@@ -266,6 +267,17 @@ __host__ __device__ constexpr size_t part_floats() {
 template <int RT, int D>
 __device__ __forceinline__ float* part_slot(const Attn& a, int cta, int which) {
     return a.part + (size_t)(2 * cta + which) * part_floats<RT, D>();
+}
+
+// Weights p = 2^(s - m) of fp16 products are lifted by a power of two, 2^lift p,
+// whose greatest value is the 2^15 that fp16 still holds: the type ends at 2^-24
+// below, not at 2^-126 as fp32 and bf16 do, and unlifted a key 17 nats behind the
+// largest lost all of its weight in the products but none in the sum (over 2^20 such
+// keys 3% of the output).  The sum is taken over lifted weights too, in the partial
+// sums as well, so the division takes the lift out.  above: log2 of the greatest p.
+template <class T>
+__device__ constexpr float lift(int above) {
+    return std::is_same<T, __half>::value ? float(15 - above) : 0.f;
 }
 
 __device__ __forceinline__ float ex2(float x) {

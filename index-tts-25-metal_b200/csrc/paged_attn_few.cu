@@ -18,7 +18,8 @@
 // its left operand in.
 //
 // 16 bits: m16n8k16.  p is split into a 16-bit head and a 16-bit rest (two
-// products), so that rounding p adds nothing to the rounding of the output.
+// products), so that 2^-18 of it is lost at most, far below the rounding of the
+// output; in fp16, where p is lifted to 2^15, 2^-40 of the largest weight at most.
 // 32 bits: m16n8k8 on TF32 with every operand split x = hi + lo and three
 // products hi hi + hi lo + lo hi, as in gemm_tma.cu; scores are summed in four
 // accumulators.  The dimensions (keys, for the second product) are dealt to the
@@ -304,6 +305,7 @@ struct Rows {
             moved |= mn > m[j];
             ref[j] = mn == -INFINITY ? 0.f : mn;
             cor[j] = ex2(m[j] - ref[j]);
+            ref[j] -= lift<T>(0);
             m[j] = mn;
             l[j] *= cor[j];
         }

@@ -13,9 +13,9 @@
 // the tensor core 1500 (a product of 64 keys takes it as long as one of 128, since
 // Q is read again from shared memory), the chain of a tile takes the rest of the
 // way.  With P over the scores, units of 128 keys: 3850 for 128.
-// The output is rescaled only when the maximum has grown by 2^8 or more since the last
-// time: P stays below 2^8, far from the 16-bit types' limits, and the division at the
-// end takes the same maximum out again.
+// The output is rescaled only when the maximum has grown by more than 2^8 (fp16: 2^4)
+// since the last time: P stays below that, within the 16-bit types' limits, and the
+// division at the end takes the same maximum out again.
 // Tried and left, as none was faster: a part of the exponentials by a polynomial on
 // the FMA units; weights with the last unit's maximum beside this unit's; two threads
 // a row (four softmax warpgroups); the tiles' exponentials in turns or out of step;
@@ -38,8 +38,8 @@
 // Tensor memory: S of the tiles, P of the tiles, O of the tiles.
 //
 // P is rounded to the 16-bit type once (V's type: the products take one type);
-// the sum is taken over the unrounded values.  That rounding is of the size of
-// the output's own, and averages over the keys.
+// the sum is taken over the unrounded values.  That rounding is of the size of the
+// output's own at most, and less where the keys' roundings differ.
 //
 // Masks are applied only in units that hold a masked key for some row of the
 // warp.  V rows behind the item's last key are zeroed in shared memory before
@@ -68,7 +68,11 @@ static_assert(2 * kSoftmaxRegs + kOtherRegs == 3 * kRegsLaunch && kSoftmaxRegs >
               "more would wait for ever; inc does not lower, dec does not raise");
 constexpr int kTileCtas = 148;
 constexpr int kTileItem = 1;  // what an item costs besides its units, in units
-constexpr float kGrow = 8.f;  // log2 of the growth of the maximum that is let pass
+// log2 of the growth of the maximum that is let pass.  fp16 has 15 octaves above 1 to share out between it and the
+// lift of the weights, which keeps small ones: 2^-25 2^-11 of the maximum is where they end (chunks of 512..1024 rows
+// over 1024..8192 keys: 2^8 and no lift 291 us, 2^4 and 2^11 292).
+template <class T>
+constexpr int kGrow = std::is_same<T, __half>::value ? 4 : 8;
 // Keys over which tensor memory sums up an item's output.  The tensor core's accumulation does not round to nearest:
 // with 2^20 keys at a stretch the result came out 6e-3 short, with 2^14 1e-4.  Then the sums so far go to the item's
 // slot of the workspace, where they are added up in fp32 (148 items of 2^17 keys 2.12 ms at a stretch, 2.18 ms so).
@@ -562,7 +566,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         l = 0.f;
                     }
                 }
-                const bool grow = top > m + kGrow || (m == -INFINITY && top > m);
+                const bool grow = top > m + float(kGrow<T>) || (m == -INFINITY && top > m);
                 if (__any_sync(0xffffffffu, grow)) {
                     const float mn = fmaxf(m, top), f = mn == -INFINITY ? 1.f : ex2(m - mn);
                     m = mn;
@@ -579,7 +583,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         }
                     }
                 }
-                const float ref = m == -INFINITY ? 0.f : -m;
+                const float ref = m == -INFINITY ? 0.f : lift<T>(kGrow<T>) - m;
                 const float2 sc = make_float2(a.scale2, a.scale2), rf = make_float2(ref, ref);
                 float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll

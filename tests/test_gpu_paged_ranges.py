@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_paged import DEV, F32, ints
+from test_gpu_paged import BF16, DEV, F16, F32, ints
 
 pytestmark = pytest.mark.gpu
 
@@ -49,3 +49,34 @@ def test_attention_fp32_sums_over_many_keys(paged, value, fresh, dim, requests):
             got, want = one_key_ahead(paged, F32, n, fresh, dim, requests, lead, top, value)
             tol = want * (2 * (2.0 ** -16 + 2.0 ** -18 + 2.0 ** -18) + 2.0 ** -17 + 2.0 ** -24)
             assert bool(((got - want).abs() <= tol).all()), float((got / want - 1).abs().max())
+
+
+# Weights: half a step of the type where the products take them rounded, and of fp16, whose steps end, half of the
+# last (2^-25 of the largest weight's 2^11) for every key.  Half a step for the output.  Sums over at most 2^14 keys at
+# a stretch: 2^-13 and 2^-18 (see test_attention_long_sums).  The exponent, up to 2^5 in size: 2^-24 of it from each
+# of two roundings, and 2^-22 from the exponential itself: 2^-17 in all.
+def allowed(dtype, n, want):
+    last = n * 2.0 ** -36 if dtype is F16 else 0.0
+    return want * (torch.finfo(dtype).eps + 2.0 ** -13 + 2.0 ** -18 + 2.0 ** -17) + last
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("fresh,dim,requests", [(1, 128, 1), (1, 64, 150), (8, 128, 300), (300, 128, 2), (300, 64, 160)])
+@pytest.mark.parametrize("n", [131089, 2 ** 19 + 77])
+def test_attention_small_weights_stay_in_the_mean(paged, n, fresh, dim, requests, dtype):
+    """Values that are all 1 have the mean 1, however far one key's score is ahead."""
+    for lead in (17.2, 17.35):
+        for top in (0, n - fresh):
+            got, want = one_key_ahead(paged, dtype, n, fresh, dim, requests, lead, top, 1.0)
+            assert float((got - want).abs().max()) <= float(allowed(dtype, n, want).max())
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("fresh,dim", [(1, 64), (1, 128), (16, 128), (40, 64), (300, 128)])
+@pytest.mark.parametrize("lead", [12, 14, 15, 16, 17, 18])
+def test_attention_small_weights_beside_a_key_without_value(paged, lead, fresh, dim, dtype):
+    """The key that is ahead has a value of 0, so the others' weights are all there is."""
+    n = 100_003
+    for top in (0, 4321, n - fresh):
+        got, want = one_key_ahead(paged, dtype, n, fresh, dim, 1, float(lead), top, 0.0)
+        assert bool(((got - want).abs() <= allowed(dtype, n, want)).all()), float((got / want - 1).abs().max())
