@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <utility>
 
 #include "model.hpp"
@@ -206,6 +207,27 @@ cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, int block, size_t smem, 
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);
+}
+
+// Allows a kernel `bytes` of dynamic shared memory, once per device.  regs: what a
+// kernel that shares out its registers (setmaxnreg) has to have been compiled to;
+// with fewer the shares would wait for ever.
+template <auto kKernel>
+cudaError_t allow_smem(size_t bytes, int regs = 0) {
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    if (regs) {
+        cudaFuncAttributes at{};
+        if ((e = cudaFuncGetAttributes(&at, kKernel)) != cudaSuccess) return e;
+        if (at.numRegs != regs) return cudaErrorInvalidKernelImage;
+    }
+    e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
 }
 
 }  // namespace itts

@@ -22,7 +22,6 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include <atomic>
 #include <type_traits>
 
 #include "common.cuh"
@@ -30,27 +29,6 @@
 
 namespace itts {
 namespace paged {
-
-// Allows a kernel `bytes` of dynamic shared memory, once per device.  regs: what a
-// kernel that shares out its registers (setmaxnreg) has to have been compiled to;
-// with fewer the shares would wait for ever.
-template <auto kKernel>
-cudaError_t allow_smem(size_t bytes, int regs = 0) {
-    static std::atomic<uint64_t> done{0};
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
-    if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
-    if (regs) {
-        cudaFuncAttributes at{};
-        if ((e = cudaFuncGetAttributes(&at, kKernel)) != cudaSuccess) return e;
-        if (at.numRegs != regs) return cudaErrorInvalidKernelImage;
-    }
-    e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
-    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
-    return e;
-}
 
 constexpr int kMaxCtas = 592;  // of one attention launch: 148 SMs, up to four CTAs each
 constexpr float kLog2e = 1.4426950408889634f;

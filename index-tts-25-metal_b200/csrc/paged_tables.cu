@@ -289,11 +289,9 @@ cudaError_t launch_tables(const itts_paged_tables_args& a, cudaStream_t s) {
     const int map_rows = fused ? a.rows : 0;
     const int ctas = a.requests + map_rows + a.rows / a.block_size <= kSmallWork ? 1 : kClusterCtas;
     const size_t smem = (size_t(a.requests) * 4 + 3) * sizeof(int);
-    cudaError_t e = cudaSuccess;
-    if (smem > 48 * 1024 &&
-        (e = cudaFuncSetAttribute(k_tables, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  int((ITTS_PAGED_MAX_REQUESTS * 4 + 3) * sizeof(int)))) != cudaSuccess)
-        return e;
+    // whatever the size: what a launch may use without leave is 48 KB less the kernel's static shared memory
+    cudaError_t e = allow_smem<k_tables>((size_t(ITTS_PAGED_MAX_REQUESTS) * 4 + 3) * sizeof(int));
+    if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas);
     cfg.blockDim = dim3(kTabThreads);
