@@ -475,7 +475,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         uint32_t ph_s = 0, ph_o = 0;
         bool ok = true;
         for (int i = 0, x = 0;; ++x) {
-            if (ok) ok = mbar_wait(&sm.seg_full[x % kSegments], uint32_t(x / kSegments) & 1u, &sm.abort);
+            // where its rows have no units in an item, this tile waits for the next one's while the other works on it
+            if (ok) ok = mbar_wait(&sm.seg_full[x % kSegments], uint32_t(x / kSegments) & 1u, &sm.abort, kItemLimitNs);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             const Segment& g = sm.seg[x % kSegments];
@@ -492,7 +493,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             };
             const auto since = [&](float then) { return then == m ? 1.f : ex2(then - m); };  // both may be -inf
             for (int j = 0; j < units; ++j, seen -= KU) {
-                ok = mbar_wait(&sm.s_ready[t], ph_s, &sm.abort);
+                ok = mbar_wait(&sm.s_ready[t], ph_s, &sm.abort, j == 0 ? kItemLimitNs : kWaitLimitNs);
                 ok = __all_sync(0xffffffffu, ok);
                 ph_s ^= 1u;
                 if (!ok) break;
