@@ -442,6 +442,7 @@ class CodecTiming(C.Structure):
 
 QWEN_VOCAB = 151936
 QWEN_EOS = 151643
+QWEN_MAX_GENERATE = 1024
 
 
 class QwenTiming(C.Structure):
@@ -508,10 +509,12 @@ class QwenDecoder:
         b = len(ps)
         ptrs = (C.c_void_p * max(1, b))(*[p.ctypes.data for p in ps])
         sizes = (C.c_size_t * max(1, b))(*[p.size for p in ps])
-        out = np.zeros((max(1, b), max(1, maximum)), np.uint32)
+        # the library refuses 0; a larger bound would wrap around in its uint32
+        bound = int(maximum) if 0 < maximum <= QWEN_MAX_GENERATE else 0
+        out = np.zeros((max(1, b), max(1, bound)), np.uint32)
         n, st = np.zeros(max(1, b), np.uint32), np.zeros(max(1, b), np.int32)
         self._check(self._lib.itts_qwen_generate_batch(self._h, b, C.cast(ptrs, C.c_void_p), C.cast(sizes, C.c_void_p),
-                                                       int(maximum), _ptr(out), _ptr(n), _ptr(st)))
+                                                       bound, _ptr(out), _ptr(n), _ptr(st)))
         return [GenerationResult(out[i, :n[i]].copy(), bool(st[i])) for i in range(b)]
 
     def cached_tokens(self) -> int:
