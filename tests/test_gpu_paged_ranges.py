@@ -1,12 +1,13 @@
 """The paged attention at the ends of its numeric ranges, on a B200: weights far
-below the largest, against the definition in 64 bits."""
+below the largest, large scores, maxima that keep growing, against the definition
+in 64 bits."""
 import importlib
 import math
 
 import pytest
 import torch
 
-from test_gpu_paged import BF16, DEV, F16, F32, ints
+from test_gpu_paged import BF16, DEV, F16, F32, Step, ints
 
 pytestmark = pytest.mark.gpu
 
@@ -80,3 +81,54 @@ def test_attention_small_weights_beside_a_key_without_value(paged, lead, fresh, 
     for top in (0, 4321, n - fresh):
         got, want = one_key_ahead(paged, dtype, n, fresh, dim, 1, float(lead), top, 0.0)
         assert bool(((got - want).abs() <= allowed(dtype, n, want)).all()), float((got / want - 1).abs().max())
+
+
+def check_large_scores(s, out, scale):
+    """As Step.check, with the exponents' errors by their size: of |s| log2(e), three roundings of the scale's product
+    (to both ends of a difference), one each of the maximum and its lift, two of the difference and of a rescaling:
+    12 2^-24 |s| of a weight, and that above and below the line.  fp16 weights end as in allowed()."""
+    u, half = 2.0 ** -24, 0.0 if s.dtype is F32 else torch.finfo(s.dtype).eps / 2
+    group = s.heads // s.kv
+    for b, n in enumerate(s.lens_h):
+        rows = slice(s.start[b], s.start[b + 1])
+        f = rows.stop - rows.start
+        seen = torch.arange(n, device=DEV)[None, :] <= (n - f + torch.arange(f, device=DEV))[:, None]
+        for h in range(s.heads):
+            q, k, v = s.q[rows, h].double(), s.k[b][:, h // group].double(), s.v[b][:, h // group].double()
+            x = (q @ k.T * scale).masked_fill(~seen, -torch.inf)
+            p = torch.softmax(x, -1)
+            want, a = p @ v, p @ v.abs()
+            products = (q.abs() @ k.abs().T * abs(scale)).masked_fill(~seen, 0.0).amax(-1, keepdim=True)
+            largest = x.masked_fill(~seen, 0.0).abs().amax(-1, keepdim=True)
+            rel = half + 2 * (s.dim + 2) * u * products + 24 * u * largest + 2 * n * u + 2.0 ** -20
+            tol = torch.finfo(s.dtype).eps / 2 * want.abs() + a * rel * 1.01
+            if s.dtype is F16:
+                tol = tol + n * 2.0 ** -36 * v.abs().max()
+            err = (out[rows, h].double() - want).abs()
+            assert bool((err <= tol).all()), (b, h, float((err / tol).max()))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("fresh", [1, 4, 8, 33, 200])
+@pytest.mark.parametrize("scale,qscale", [(3.0, 4.0), (-3.0, 4.0), (0.5, 30.0)])
+def test_attention_scores_of_hundreds(paged, scale, qscale, fresh, dim, dtype):
+    s = Step([(fresh, 200), (fresh, 1900)], 4, 2, dim, bs=64, dtype=dtype, qscale=qscale)
+    check_large_scores(s, s.run(paged, scale=scale), scale)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("fresh,dim", [(1, 128), (3, 64), (8, 64), (40, 64), (300, 128), (300, 64)])
+@pytest.mark.parametrize("step", [1, 3, 4, 5, 7, 8, 9, 15, -4, -9])
+def test_attention_maxima_that_grow(paged, step, fresh, dim, dtype):
+    """Scores that rise (or fall) by `step` octaves from each 64 keys to the next: below, at and above the growth that
+    the tile kernels let pass before they rescale."""
+    s = Step([(fresh, 1000)], 4, 2, dim, bs=32, dtype=dtype, qscale=0.3)
+    s.q[:, :, 0] = 1.0
+    n = s.lens_h[0]
+    rise = (step * (torch.arange(n, device=DEV) // 64)).to(dtype)
+    s.k[0][:, :, 0] = rise[:, None]
+    for j in range((n + 31) // 32):
+        s.kc[s.table[0, j].item(), :min(32, n - 32 * j)] = s.k[0][32 * j:min(n, 32 * j + 32)]
+    scale = math.log(2.0)
+    check_large_scores(s, s.run(paged, scale=scale), scale)
