@@ -16,7 +16,8 @@
 // An item that ends up with several CTAs leaves partial sums in the workspace,
 // two slots a CTA (slot 0: the item its share begins inside of; slot 1: the
 // item that begins in it and goes on in the next); k_join adds them up in CTA
-// order, so results do not depend on timing.
+// order, so results do not depend on timing.  Within a share sums of long items
+// meet there, too, stretch by stretch.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -245,6 +246,27 @@ __host__ __device__ constexpr size_t part_floats() {
 template <int RT, int D>
 __device__ __forceinline__ float* part_slot(const Attn& a, int cta, int which) {
     return a.part + (size_t)(2 * cta + which) * part_floats<RT, D>();
+}
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+// 16 bytes to shared memory; the first `bytes` of them are read, the rest is zeros.
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+// Two values in 16 bits.
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float x, float y);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float x, float y) {
+    const __half2 v = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, float y) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&v);
 }
 
 // Weights p = 2^(s - m) of fp16 products are lifted by a power of two, 2^lift p,

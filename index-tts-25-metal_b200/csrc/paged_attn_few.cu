@@ -65,8 +65,6 @@ struct Few {
 };
 constexpr size_t kFewSmem = size_t(kRingBytes) * kFewWarps;
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
 // Chunk of row r that chunk c is kept at (see the reads below: every access of
 // eight lanes falls on eight different banks of 16 bytes).
 template <class T>
@@ -76,10 +74,6 @@ __device__ __forceinline__ int swz_k(int r, int c) {
 template <class T>
 __device__ __forceinline__ int swz_v(int r, int c) {
     return sizeof(T) == 4 ? c ^ (((r >> 1) & 3) << 1) : c ^ (r & 7);
-}
-
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
@@ -130,19 +124,7 @@ __device__ __forceinline__ void mma8x3(float (&d)[4], const float (&ah)[4], cons
     mma8(d, ah, h0, h1);
 }
 
-// Two values in 16 bits, and what the rounding left.
-template <class T>
-__device__ __forceinline__ uint32_t pack2(float x, float y);
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float x, float y) {
-    const __half2 v = __floats2half2_rn(x, y);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, float y) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
+// What two values in 16 bits stand for.
 template <class T>
 __device__ __forceinline__ float2 unpack2(uint32_t v);
 template <>

@@ -130,23 +130,6 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint3
         : "memory");
 }
 
-template <class T>
-__device__ __forceinline__ uint32_t pack16(float x, float y);
-template <>
-__device__ __forceinline__ uint32_t pack16<__half>(float x, float y) {
-    const __half2 v = __floats2half2_rn(x, y);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
-template <>
-__device__ __forceinline__ uint32_t pack16<__nv_bfloat16>(float x, float y) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
-
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -596,7 +579,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                             float2 y = fma2(make_float2(__uint_as_float(s[c][2 * e]), __uint_as_float(s[c][2 * e + 1])), sc, rf);
                             y = make_float2(ex2(y.x), ex2(y.y));
                             sum[e & 1] = add2(sum[e & 1], y);
-                            p[e] = pack16<T>(y.x, y.y);
+                            p[e] = pack2<T>(y.x, y.y);
                         }
                     } else {
 #pragma unroll
@@ -658,7 +641,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
                         for (int e = 0; e < 8; ++e) y[e] = l == 0.f ? 0.f : y[e] * inv;
                         *reinterpret_cast<uint4*>(dst + 32 * c + x) = make_uint4(
-                            pack16<T>(y[0], y[1]), pack16<T>(y[2], y[3]), pack16<T>(y[4], y[5]), pack16<T>(y[6], y[7]));
+                            pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7]));
                     } else {
                         float4* to = reinterpret_cast<float4*>(slot + (size_t)row * D + 32 * c + x);
                         to[0] = make_float4(y[0], y[1], y[2], y[3]);

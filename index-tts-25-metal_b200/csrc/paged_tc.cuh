@@ -10,8 +10,6 @@
 namespace itts {
 namespace paged {
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
 __device__ __forceinline__ void mbar_init(unsigned long long* bar, int count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
 }
@@ -120,13 +118,6 @@ __device__ __forceinline__ uint32_t desc_low(uint32_t addr, uint32_t lead) {
         "=r"(v[o + 19]), "=r"(v[o + 20]), "=r"(v[o + 21]), "=r"(v[o + 22]), "=r"(v[o + 23]), "=r"(v[o + 24]),       \
         "=r"(v[o + 25]), "=r"(v[o + 26]), "=r"(v[o + 27]), "=r"(v[o + 28]), "=r"(v[o + 29]), "=r"(v[o + 30]),       \
         "=r"(v[o + 31])
-#define ITTS_S32(v, o)                                                                                             \
-    "r"(v[o]), "r"(v[o + 1]), "r"(v[o + 2]), "r"(v[o + 3]), "r"(v[o + 4]), "r"(v[o + 5]), "r"(v[o + 6]),            \
-        "r"(v[o + 7]), "r"(v[o + 8]), "r"(v[o + 9]), "r"(v[o + 10]), "r"(v[o + 11]), "r"(v[o + 12]),                \
-        "r"(v[o + 13]), "r"(v[o + 14]), "r"(v[o + 15]), "r"(v[o + 16]), "r"(v[o + 17]), "r"(v[o + 18]),             \
-        "r"(v[o + 19]), "r"(v[o + 20]), "r"(v[o + 21]), "r"(v[o + 22]), "r"(v[o + 23]), "r"(v[o + 24]),             \
-        "r"(v[o + 25]), "r"(v[o + 26]), "r"(v[o + 27]), "r"(v[o + 28]), "r"(v[o + 29]), "r"(v[o + 30]),             \
-        "r"(v[o + 31])
 
 // 32 columns of this warp's 32 lanes of tensor memory: lane = row.
 template <int N>
@@ -136,14 +127,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&v)[N], int o
         "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
         : ITTS_R32(v, o)
         : "r"(addr));
-}
-template <int N>
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&v)[N], int o = 0) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
-        "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::ITTS_S32(v, o),
-        "r"(addr)
-        : "memory");
 }
 template <int N>
 __device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&v)[N]) {
@@ -174,7 +157,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[N])
         : "memory");
 }
 #undef ITTS_R32
-#undef ITTS_S32
 
 // Tensor map of a paged cache tensor: [blocks][heads][block_size][head_dim]
 // at its strides, read as boxes of up to `tokens` tokens of one block and head x
