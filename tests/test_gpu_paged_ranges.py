@@ -132,3 +132,68 @@ def test_attention_maxima_that_grow(paged, step, fresh, dim, dtype):
         s.kc[s.table[0, j].item(), :min(32, n - 32 * j)] = s.k[0][32 * j:min(n, 32 * j + 32)]
     scale = math.log(2.0)
     check_large_scores(s, s.run(paged, scale=scale), scale)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("fresh,dim,requests", [(1, 128, 300), (1, 64, 170), (4, 64, 170), (8, 128, 150), (16, 128, 150),
+                                                (40, 64, 149), (130, 128, 150), (300, 64, 80)])
+def test_attention_long_items(paged, fresh, dim, requests, dtype):
+    """Items whose sums meet several times within a share and across shares: random keys that all requests have in
+    common, blocks among them that the table does not name.  Each of the stretches' sums is an fp32 one, and a
+    tensor-core sum of up to 2^14 keys is off by 2^-13 of it at most (fp32: 2^-18, a unit of 64 keys)."""
+    n, bs, u = 40_077, 64, 2.0 ** -24
+    g = torch.Generator(device=DEV).manual_seed(fresh + dim)
+    blocks = (n + bs - 1) // bs
+    k = torch.randn(blocks * bs, 1, dim, generator=g, device=DEV).to(dtype)
+    v = torch.randn(blocks * bs, 1, dim, generator=g, device=DEV).to(dtype)
+    q = (torch.randn(fresh * requests, 1, dim, generator=g, device=DEV) * 2).to(dtype)
+    row = torch.arange(blocks, dtype=torch.int32, device=DEV)
+    row[3], row[300], row[555] = -1, blocks, 1 << 30
+    table = row.expand(requests, blocks).contiguous()
+    out = paged.attention(q, k.view(blocks, bs, 1, dim), v.view(blocks, bs, 1, dim), table, ints([n] * requests),
+                          ints([fresh * b for b in range(requests + 1)]), fresh)
+    j = torch.arange(n, device=DEV)
+    named = (j // bs != 3) & (j // bs != 300) & (j // bs != 555)
+    seen = (j[None, :] <= (n - fresh + torch.arange(fresh, device=DEV))[:, None]) & named
+    kd, vd, half = k[:n, 0].double(), v[:n, 0].double(), 0.0 if dtype is F32 else torch.finfo(dtype).eps / 2
+    for b in [*range(0, requests, 9), requests - 2, requests - 1]:
+        rows = slice(b * fresh, (b + 1) * fresh)
+        x = (q[rows, 0].double() @ kd.T * dim ** -0.5).masked_fill(~seen, -torch.inf)
+        p = torch.softmax(x, -1)
+        want, a = p @ vd, p @ vd.abs()
+        size = (q[rows, 0].double().abs() @ kd.abs().T).amax(-1, keepdim=True) * dim ** -0.5
+        sums = 2.0 ** -18 if dtype is F32 else 2.0 ** -13
+        rel = half + 2 * (dim + 2) * u * size + 2.0 ** -20 + 2 * (sums + 2.0 ** -16 + 2.0 ** -20)
+        tol = torch.finfo(dtype).eps / 2 * want.abs() + a * rel * 1.01
+        if dtype is F16:
+            tol = tol + n * 2.0 ** -36 * vd.abs().max()
+        err = (out[rows, 0].double() - want).abs()
+        assert bool((err <= tol).all()), (b, float((err / tol).max()))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("group", [16, 17, 64, 100, 127, 128])
+def test_attention_wide_groups(paged, group, dtype):
+    """Up to 128 query heads a key head: a token fills a tile, or does not divide it."""
+    s = Step([(1, 0), (1, 200), (3, 130), (5, -2), (0, 7), (40, 90)], 2 * group, 2, 64, bs=32, dtype=dtype, pad=2)
+    s.check(s.run(paged))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("max_fresh", [2, 40])
+def test_attention_most_requests(paged, max_fresh, dim, dtype):
+    s = Step([(i % 3, i % 7) for i in range(8192)], 1, 1, dim, bs=16, dtype=dtype, pad=1)
+    out = s.run(paged, max_fresh=max_fresh)
+    want = []
+    for b in range(8192):
+        f, n = s.fresh[b], s.lens_h[b]
+        if f:
+            x = s.q[s.start[b]:s.start[b + 1], 0].double() @ s.k[b][:, 0].double().T * dim ** -0.5
+            x = x.masked_fill(torch.ones_like(x, dtype=torch.bool).triu(n - f + 1), -torch.inf)
+            want.append(torch.softmax(x, -1) @ s.v[b][:, 0].double())
+    want, top = torch.cat(want), float(max(v.abs().max() for v in s.v if v.numel()))
+    # half a step each for weights and output; scores of up to 2^5: their products' roundings and the exponent, 2^-14
+    eps = 0.0 if dtype is F32 else torch.finfo(dtype).eps
+    assert float((out[:len(want), 0].double() - want).abs().max()) <= top * (eps + 2.0 ** -14)
+    assert bool((out[len(want):] == 5).all())
