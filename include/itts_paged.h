@@ -64,6 +64,9 @@ const char* itts_paged_last_error(void);
  * timing.  A block id that is handed out is not erased from the free list; the
  * entries at and above the count mean nothing.
  *
+ * Entries of the table that a request keeps are not checked: a row whose entry
+ * is outside 0 .. blocks - 1 gets the slot -1, which the append leaves out.
+ *
  * If a status bit is set nothing is taken or given: lens = cached (q_start all
  * 0, slots all -1, positions all 0), free_out = free_in, and the table is as
  * it was; free_list entries above the count may have been written. */
@@ -130,16 +133,22 @@ int itts_paged_append(int device, const itts_paged_append_args* args, void* stre
  * h / (q_heads / heads).
  *   out = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q . k_j - max)
  * A row that sees no key (position < 0) is written as zeros.  Rows before
- * q_start[0] and from q_start[requests] on are left as they were.  Scores, the
- * softmax and all sums are held in fp32.
+ * q_start[0] and from q_start[requests] on are left as they were.
+ *
+ * Scores, maxima and sums are held in fp32 and a 16-bit output is rounded once.
+ * Where max_fresh * q_heads / heads is more than 16, the 16-bit types' weights
+ * p_j are rounded to the type too before they multiply v_j (not for their sum;
+ * by half a step, up to the output's own rounding), and their products are added
+ * up by the tensor core, which does not round to nearest (up to 2^-13 of a sum).
  *
  * What lies in the cache behind a request's length, or in blocks that its
  * table does not name, never reaches the output, NaN and infinities included.
  * A table entry outside 0 .. blocks - 1 is not followed: its keys count as not
  * seen, as do the keys behind the table's last column.  q_start values are
- * clamped to 0 .. rows.  (A NaN or infinity in a key or value makes every row
- * that sees it NaN or infinite; in the value row of a later row of the same
- * chunk it may reach the chunk's earlier rows, too.)
+ * clamped to 0 .. rows.  (A NaN in a key makes every row that sees it NaN, one in
+ * a value the row's output at its dimension.  An infinity may make such a row NaN or infinite; a key whose score it
+ * makes -inf may count as not seen.  Either in the value row of a later row of
+ * the same chunk may reach the chunk's earlier rows, too.)
  *
  * Work beyond all measure is not begun: if the lengths ask for more than 2^29
  * tiles (of 1 to 128 rows by 32 to 128 keys) per CTA, which is minutes, every

@@ -54,11 +54,15 @@ int itts_qwen_generate(itts_qwen_ctx* ctx, const uint32_t* ids, size_t n, uint32
  * its ids go to out[i * maximum ..), their number to n_out[i], and stopped[i]
  * says whether the last one is EOS (a run of `maximum` ids without EOS is no
  * failure here).  Every prompt is checked as generate checks it before any runs.
+ * Its ids are those that generate selects for it alone, unless two logits lie
+ * within the rounding of one another (the two sum in different orders).
  * No counterpart in the reference, which has one sequence per decoder.
  *
  * Up to 16 prompts are in flight, a finished one's place goes to the next.  Their
  * keys and values share one paged cache (itts_paged.h); a step takes up to 1024
- * rows: one for each prompt that is generating, chunks of the others.  The
+ * rows: one for each prompt that is generating, chunks of the others.  A step
+ * costs about 4 ms and reads the vocabulary table once per generating prompt, so
+ * that generate one by one is faster for up to four prompts.  The
  * sequence of prefill / step / generate is left as it was. */
 int itts_qwen_generate_batch(itts_qwen_ctx* ctx, size_t n, const uint32_t* const* ids, const size_t* n_ids,
                              uint32_t maximum, uint32_t* out, uint32_t* n_out, int32_t* stopped);

@@ -504,7 +504,8 @@ class QwenDecoder:
     def generate_batch(self, prompts, maximum: int = 1024) -> list:
         """generate() for independent prompts at once, up to 16 in flight over
         one paged cache (itts_qwen_generate_batch): one GenerationResult per
-        prompt, ``stopped`` where its last id is EOS."""
+        prompt, ``stopped`` where its last id is EOS.  Faster than generate()
+        one by one from about eight prompts on."""
         ps = [_u32(p) for p in prompts]
         b = len(ps)
         ptrs = (C.c_void_p * max(1, b))(*[p.ctypes.data for p in ps])
